@@ -389,6 +389,41 @@ int gq_unpack_dequant(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp,
                       const int32_t* g_idx, float* dequant, uint8_t* codes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Products with packed weights (the reference only multiplies dequantized
+ * floats, quant.py:37):
+ *   y[t, r] = sum_c x[t, c] * (code[r, c] + qmin - zero[r, g]) * scale[r, g],
+ * g the group of column c.
+ *
+ * gq_linear_layout lays one weight out for gq_linear, once.  packed, scales,
+ * zeros as gq_pack_codes / gq_gptq_sweep write them.  The caller chooses the
+ * positions: k of them (a multiple of 128), kmap [k] int32 = the column at
+ * each position or -1 for padding, every column exactly once, every granule
+ * (32, 64 or 128 consecutive positions) inside one group;
+ * granule_group [k / granule] int32 = its group, or -1 where it holds padding
+ * alone.  qw: ceil(m / 16) * 16 * k * W / 32 words with W = 4 for
+ * bits <= 4 and 8 otherwise; params: ceil(m / 16) * 16 * (k / granule) pairs
+ * of floats; *bad (device int): bit 0 = a zero whose offset zero - qmin is
+ * not a whole number of 0 .. 2^bits - 1, bit 1 = a scale that is not finite
+ * (the layout is then not to be used).
+ *
+ * gq_linear: x [tokens, n] (ldx) of dtype 0 = float32, 1 = bf16, 2 = fp16,
+ * y [tokens, m] (ldy) of the same type; qw and params 16-byte aligned;
+ * direct = 1 when kmap is the identity with k == n (16-bit x is then read in
+ * place if it is 16-byte aligned with ldx % 8 == 0, and needs no workspace).  bits, granule and k as laid out.  Products are
+ * summed in float32 in a fixed order and rounded once; float32 x runs as three
+ * exact bf16 terms.  x and y must not overlap.  workspace: 256-byte aligned,
+ * gq_linear_workspace_size(tokens, k, dtype) bytes. */
+int gq_linear_layout(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp, int bits, int sym,
+                     const float* scales, const float* zeros, int64_t n_groups,
+                     const int32_t* kmap, int64_t k, const int32_t* granule_group, int granule,
+                     uint32_t* qw, float* params, int* bad, void* stream);
+int64_t gq_linear_workspace_size(int64_t tokens, int64_t k, int dtype);
+int gq_linear(const uint32_t* qw, const float* params, const int32_t* kmap, int64_t m, int64_t n,
+              int64_t k, int bits, int granule, int direct, const void* x, int dtype,
+              int64_t tokens, int64_t ldx, void* y, int64_t ldy, void* workspace,
+              int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * gptq_ref.py:95-99 (jnp.linalg.eigh of the Hessian in process_hessian's
  * eigh branch): symmetric eigendecomposition by parallel cyclic Jacobi.
  *

@@ -7,6 +7,7 @@ caller's container: numpy in -> numpy out, torch in -> torch (on the device).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import numpy as np
@@ -54,6 +55,16 @@ def ptr(t) -> ctypes.c_void_p:
 
 def stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context that makes ``device`` current (nothing to do when it is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(device)
 
 
 def empty(shape, dtype=torch.float32) -> torch.Tensor:

@@ -35,6 +35,11 @@ SIGNATURES = {
     "gq_pack_codes": (c_int, [_P, c_int64, c_int64, c_int64, c_int, _P, c_int64, _P]),
     "gq_unpack_dequant": (c_int, [_P, c_int64, c_int64, c_int64, c_int, c_int, _P, _P, c_int64,
                                   _P, _P, _P, _P]),
+    "gq_linear_layout": (c_int, [_P, c_int64, c_int64, c_int64, c_int, c_int, _P, _P, c_int64, _P,
+                                 c_int64, _P, c_int, _P, _P, _P, _P]),
+    "gq_linear_workspace_size": (c_int64, [c_int64, c_int64, c_int]),
+    "gq_linear": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int, c_int, c_int, _P, c_int,
+                          c_int64, c_int64, _P, c_int64, _P, c_int64, _P]),
     "gq_nccl_unique_id": (c_int, [_P, c_int64]),
     "gq_handle_create": (c_int, [c_int, _P, ctypes.POINTER(_P)]),
     "gq_handle_create_nccl": (c_int, [c_int, _P, c_int, c_int, ctypes.POINTER(_P)]),

@@ -1,0 +1,193 @@
+"""Linears that run on packed weights.
+
+The reference stops at dequantized floats (``quant.py:37``), and
+``packing.dequantize`` turns a packed layer back into them.  This module
+multiplies with the packed form: ``prepare_linear`` lays a
+:class:`packing.PackedLinear` out once for the tensor cores
+(``gq_linear_layout``), ``packed_matmul`` computes ``x @ W.T`` from it
+(``gq_linear``) for one token or thousands, and :class:`QuantLinear` is the
+module form.  Weights are not rounded on the way: whole-number codes are
+multiplied with x on the tensor cores, and each group's float32 sum is scaled
+once.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _arrays as A
+from . import _lib
+from .packing import PackedLinear
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+@dataclass(frozen=True)
+class PreparedLinear:
+    """Packed weights laid out for ``packed_matmul`` (see ``gq_linear_layout``)."""
+    qweight: torch.Tensor   # laid-out codes, int32 words
+    params: torch.Tensor    # [row blocks, granules, 16, 2] float32: scale, offset
+    kmap: torch.Tensor      # [k] int32: original column of each position, -1 for padding
+    m: int                  # out_features
+    n: int                  # in_features
+    k: int                  # positions
+    bits: int
+    granule: int            # columns that share one scale in the layout
+    direct: bool            # positions are the columns in their own order
+
+    @property
+    def device(self) -> torch.device:
+        return self.qweight.device
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.qweight, self.params, self.kmap))
+
+
+def _positions(g_idx: torch.Tensor, n_groups: int):
+    """(granule, k, kmap, granule_group) of the column groups ``g_idx``: columns
+    in group order, every group padded to whole granules, k a multiple of 128."""
+    n = g_idx.numel()
+    g = g_idx.long()
+    counts = torch.bincount(g, minlength=n_groups)
+    need = {}
+    for gr in (128, 64, 32):
+        need[gr] = int(((counts + gr - 1) // gr).sum()) * gr
+    # the widest granule that pads no more than the narrowest: fewer scales to
+    # read and fewer sums to scale
+    granule = next(gr for gr in (128, 64, 32) if need[gr] <= need[32])
+    k = -(-max(need[granule], 1) // 128) * 128
+    grans = (counts + granule - 1) // granule
+    order = torch.argsort(g, stable=True)
+    first = torch.cumsum(counts, 0) - counts          # of the group, among sorted columns
+    base = (torch.cumsum(grans, 0) - grans) * granule  # of the group, among positions
+    pos = base[g[order]] + torch.arange(n, device=g.device) - first[g[order]]
+    kmap = torch.full((k,), -1, dtype=torch.int32, device=g.device)
+    kmap[pos] = order.to(torch.int32)
+    gg = torch.full((k // granule,), -1, dtype=torch.int32, device=g.device)
+    filled = torch.repeat_interleave(torch.arange(n_groups, device=g.device), grans)
+    gg[:filled.numel()] = filled.to(torch.int32)
+    return granule, k, kmap, gg
+
+
+def prepare_linear(p: PackedLinear) -> PreparedLinear:
+    """Lay ``p`` out for ``packed_matmul`` on the current device (once per weight).
+
+    Raises ``ValueError`` for shapes that do not fit together, groups outside
+    the scales, zeros that are not whole numbers of the code range (the
+    quantizers here only write those) and scales that are not finite."""
+    A.require_cuda()
+    bits, n = int(p.bits), int(p.n)
+    words = _lib.lib().gq_packed_words(n, bits)
+    if words < 0 or (p.sym and bits < 2):
+        raise ValueError(f"bits must be 1..8 (2..8 symmetric), got {bits}")
+    if n < 1:
+        raise ValueError(f"in_features must be positive, got {n}")
+    if p.qweight.dim() != 2 or p.qweight.dtype != torch.int32 or p.qweight.shape[1] < words:
+        raise ValueError(f"qweight must be int32 [m, {words}], got {p.qweight.dtype} "
+                         f"{tuple(p.qweight.shape)}")
+    m = p.qweight.shape[0]
+    if p.scales.dim() != 2 or p.scales.shape != p.zeros.shape or p.scales.shape[0] != m:
+        raise ValueError(f"scales and zeros must be [m, groups] with m = {m}, got "
+                         f"{tuple(p.scales.shape)} and {tuple(p.zeros.shape)}")
+    if tuple(p.g_idx.shape) != (n,):
+        raise ValueError(f"g_idx must be [{n}], got {tuple(p.g_idx.shape)}")
+    q, g_idx = p.qweight.cuda().contiguous(), p.g_idx.cuda()
+    s, z = A.to_device(p.scales), A.to_device(p.zeros)
+    lo, hi = (int(v) for v in torch.aminmax(g_idx))
+    if lo < 0 or hi >= s.shape[1]:
+        raise ValueError(f"g_idx must lie in [0, {s.shape[1]}), got {lo} .. {hi}")
+    granule, k, kmap, gg = _positions(g_idx, s.shape[1])
+    blocks = -(-m // 16)
+    qw = torch.empty((blocks * 16 * k * (4 if bits <= 4 else 8) // 32,), dtype=torch.int32,
+                     device="cuda")
+    params = torch.empty((blocks, k // granule, 16, 2), dtype=torch.float32, device="cuda")
+    bad = torch.empty((1,), dtype=torch.int32, device="cuda")
+    _lib.call("gq_linear_layout", A.ptr(q), m, n, q.shape[1], bits, int(p.sym), A.ptr(s), A.ptr(z),
+              s.shape[1], A.ptr(kmap), k, A.ptr(gg), granule, A.ptr(qw), A.ptr(params), A.ptr(bad),
+              A.stream())
+    fault = int(bad.item())
+    if fault & 1:
+        raise ValueError(f"zeros must be whole numbers inside the {bits}-bit code range")
+    if fault & 2:
+        raise ValueError("scales must be finite")
+    direct = k == n and bool((kmap == torch.arange(k, device="cuda", dtype=torch.int32)).all())
+    return PreparedLinear(qw, params, kmap, m, n, k, bits, granule, direct)
+
+
+def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
+    """``x @ W.T`` for ``x`` [..., n] (float32, bf16 or fp16) -> [..., m] of x's type.
+
+    Products are summed in float32 (float32 x loses no bits: it runs as three
+    exact bf16 terms) and rounded once.  numpy in -> numpy out.  ``out``, if
+    given, is a contiguous tensor of the result's shape and type that does not
+    share memory with ``x``."""
+    if A.is_host(x):
+        return A.like_input(packed_matmul(A.to_device(x), w), x)
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != w.n:
+        raise ValueError(f"x must be [..., {w.n}], got {tuple(x.shape)}")
+    if x.device != w.qweight.device:
+        raise ValueError(f"x is on {x.device}, the weights on {w.qweight.device}")
+    shape = (*x.shape[:-1], w.m)
+    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= w.n:
+        x2 = x
+    else:
+        x2 = x.reshape(-1, w.n).contiguous()
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif tuple(out.shape) != shape or out.dtype != x.dtype or out.device != x.device or \
+            not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {x.dtype} tensor {shape} on {x.device}")
+    elif out.numel() and x2.numel() and _overlap(out, x2):
+        raise ValueError("out shares memory with x")
+    tokens = x2.shape[0]
+    if tokens == 0 or w.m == 0:
+        return out
+    with A.on_device(x.device):
+        nbytes, ws = 0, None
+        if not (w.direct and dt and x2.data_ptr() % 16 == 0 and x2.stride(0) % 8 == 0):
+            nbytes = _lib.lib().gq_linear_workspace_size(tokens, w.k, dt)
+            ws = A.workspace(nbytes)
+        _lib.call("gq_linear", w.qweight.data_ptr(), w.params.data_ptr(), w.kmap.data_ptr(), w.m,
+                  w.n, w.k, w.bits, w.granule, int(w.direct), x2.data_ptr(), dt, tokens,
+                  x2.stride(0), out.data_ptr(), w.m, None if ws is None else ws.data_ptr(), nbytes,
+                  A.stream())
+    return out
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    def span(t):
+        last = sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+class QuantLinear(torch.nn.Module):
+    """A bias-free linear on packed weights (inference only)."""
+
+    def __init__(self, p: PackedLinear | PreparedLinear):
+        super().__init__()
+        self.weights = p if isinstance(p, PreparedLinear) else prepare_linear(p)
+
+    @property
+    def in_features(self) -> int:
+        return self.weights.n
+
+    @property
+    def out_features(self) -> int:
+        return self.weights.m
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return packed_matmul(x, self.weights)
+
+    def extra_repr(self) -> str:
+        w = self.weights
+        return f"in_features={w.n}, out_features={w.m}, bits={w.bits}"
+
+
+__all__ = ["PreparedLinear", "QuantLinear", "packed_matmul", "prepare_linear"]
