@@ -424,6 +424,25 @@ int gq_linear(const uint32_t* qw, const float* params, const int32_t* kmap, int6
               int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Rotary positions of queries and keys (the model code around the reference
+ * leaves them to its model library).  q [batch, heads, seq, head_dim] and k
+ * [batch, kv_heads, seq, head_dim] (kv_heads = 0: none) of dtype 0 = float32,
+ * 1 = bf16, 2 = fp16; strides (HOST, 12 values, elements): batch, head and
+ * position of q, q_out, k, k_out; components are contiguous.  Pairs of the
+ * first rotary_dim components, (i, i + rotary_dim / 2) or with interleaved
+ * (2 i, 2 i + 1), are turned by position * turns[i] and multiplied by factor;
+ * the rest is copied.  turns [rotary_dim / 2]: 2^-64ths of a full turn per
+ * position, the product wraps.  positions: int64 (or int32) [batch, seq] with
+ * row stride position_stride (0: one row for all).  transpose = 1 turns back
+ * (the gradient's map).  Outputs may be the inputs; other overlap is not
+ * allowed.  Computed in float32, rounded once. */
+int gq_rotary(const void* q, void* q_out, int64_t heads, const void* k, void* k_out,
+              int64_t kv_heads, const int64_t* strides, const void* positions,
+              int64_t position_stride, int positions_are_int32, const int64_t* turns,
+              int64_t batch, int64_t seq, int head_dim, int rotary_dim, int interleaved,
+              float factor, int transpose, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------
  * gptq_ref.py:95-99 (jnp.linalg.eigh of the Hessian in process_hessian's
  * eigh branch): symmetric eigendecomposition by parallel cyclic Jacobi.
  *

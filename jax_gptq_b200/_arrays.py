@@ -67,6 +67,54 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors may share memory.  Views side by side in one buffer
+    (heads of a joint projection, columns of one matrix) are told apart by the
+    outer dimensions they have in common; what is not decided counts as shared."""
+    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
+        return False
+    da = sorted((s * a.element_size(), n) for n, s in zip(a.shape, a.stride()) if n > 1)
+    db = sorted((s * b.element_size(), n) for n, s in zip(b.shape, b.stride()) if n > 1)
+    common = []  # outer dimensions, outermost first
+    while True:
+        if _apart(a, b, da, db, common):
+            return False
+        if not (da and db and da[-1] == db[-1]):
+            return True
+        common.append(da.pop())
+        db.pop()
+
+
+def _apart(a, b, da, db, common) -> bool:
+    """Whether the inner blocks ``da`` and ``db`` of two tensors lie apart, in
+    windows that the ``common`` outer strides never bring over each other."""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    a1 = a0 + sum(s * (n - 1) for s, n in da) + a.element_size()
+    b1 = b0 + sum(s * (n - 1) for s, n in db) + b.element_size()
+    whole = sum(s * (n - 1) for s, n in common)
+    if a1 + whole <= b0 or b1 + whole <= a0:
+        return True
+    if a0 < b1 and b0 < a1:
+        return False
+    width = max(a1, b1) - min(a0, b0)
+    for s, n in reversed(common):
+        if s < width:
+            return False
+        width += s * (n - 1)
+    return True
+
+
+def distinct_elements(t: torch.Tensor) -> bool:
+    """Whether no two elements of ``t`` share memory, judged by its strides:
+    each is at least the span of the ones below it."""
+    span = 1
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s < span:
+            return False
+        span = s * (n - 1) + span
+    return True
+
+
 def empty(shape, dtype=torch.float32) -> torch.Tensor:
     return torch.empty(shape, dtype=dtype, device="cuda")
 

@@ -142,7 +142,7 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     elif tuple(out.shape) != shape or out.dtype != x.dtype or out.device != x.device or \
             not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {x.dtype} tensor {shape} on {x.device}")
-    elif out.numel() and x2.numel() and _overlap(out, x2):
+    elif A.overlap(out, x2):
         raise ValueError("out shares memory with x")
     tokens = x2.shape[0]
     if tokens == 0 or w.m == 0:
@@ -157,14 +157,6 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
                   x2.stride(0), out.data_ptr(), w.m, None if ws is None else ws.data_ptr(), nbytes,
                   A.stream())
     return out
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    def span(t):
-        last = sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
 
 
 class QuantLinear(torch.nn.Module):
