@@ -443,6 +443,28 @@ int gq_rotary(const void* q, void* q_out, int64_t heads, const void* k, void* k_
               float factor, int transpose, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Choice of the next token (beside eval.py:9-22, which scores given tokens on
+ * the same logits).  logits [rows, vocab] (ld) of dtype 0 = float32, 1 = bf16,
+ * 2 = fp16, vocab <= 2^20; NaN and -inf are excluded.  Each setting is one
+ * value (kind 0) or one per row (kind 1 float32, 2 float64, 3 int32, 4 int64);
+ * u has one per row (kind 1 or 2).  Tokens are ordered by logit, equal ones by
+ * index, with e = exp((logit - max) / temperature):
+ *   top_k >= 1 keeps the first top_k (0 or below: all); top_p < 1 keeps, of
+ *   those, the ones before which less than top_p of their mass lies; min_p > 0
+ *   keeps, of those, the ones with e >= min_p; the first is always kept.
+ * tokens[row] = the smallest index i for which the sum of e over kept tokens
+ * 0 .. i exceeds u times the sum over all kept (u of 1 or more: the last kept);
+ * logprobs[row] (or NULL) = log of its share of the kept mass.  temperature
+ * not above 0: the first largest logit, logprob 0.  A row without a token: -1
+ * and -inf.  Sums are of whole numbers of 2^-45 (2^-42 for the largest
+ * vocabularies) of the largest term, independent of any order. */
+int gq_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+              const void* u, int u_kind, const void* temperature, int temperature_kind,
+              double temperature_value, const void* top_k, int top_k_kind, double top_k_value,
+              const void* top_p, int top_p_kind, double top_p_value, const void* min_p,
+              int min_p_kind, double min_p_value, int64_t* tokens, float* logprobs, void* stream);
+
+/* ------------------------------------------------------------------------
  * gptq_ref.py:95-99 (jnp.linalg.eigh of the Hessian in process_hessian's
  * eigh branch): symmetric eigendecomposition by parallel cyclic Jacobi.
  *

@@ -42,6 +42,8 @@ SIGNATURES = {
                           c_int64, c_int64, _P, c_int64, _P, c_int64, _P]),
     "gq_rotary": (c_int, [_P, _P, c_int64, _P, _P, c_int64, _P, _P, c_int64, c_int, _P, c_int64,
                           c_int64, c_int, c_int, c_int, c_float, c_int, c_int, _P]),
+    "gq_sample": (c_int, [_P, c_int, c_int64, c_int64, c_int64, _P, c_int, _P, c_int, c_double, _P,
+                          c_int, c_double, _P, c_int, c_double, _P, c_int, c_double, _P, _P, _P]),
     "gq_nccl_unique_id": (c_int, [_P, c_int64]),
     "gq_handle_create": (c_int, [c_int, _P, ctypes.POINTER(_P)]),
     "gq_handle_create_nccl": (c_int, [c_int, _P, c_int, c_int, ctypes.POINTER(_P)]),
