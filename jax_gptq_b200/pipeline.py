@@ -16,6 +16,13 @@ model walk).  ``quantize_stack`` is that walk for a Llama-style stack:
 * with a checkpoint directory, blocks already on disk are reloaded instead of
   re-quantized, so an interrupted run resumes where it stopped.
 
+A quantized stack runs from its packed layer files: ``attach_packed`` puts
+``linear.QuantLinear`` modules in the place of a stack's linears, so the walk
+of the next block, a perplexity window or a decode step multiplies with the
+codes themselves; ``TinyLM.generate`` decodes with a key/value cache, rotary
+positions from ``rotary.apply_rotary`` and tokens from
+``sampling.sample_tokens``.
+
 The block itself (RMSNorm, rotary attention with grouped KV heads, SwiGLU
 MLP) is plain torch: it is the model whose activations feed the kernels, not
 part of the quantization path.
@@ -31,7 +38,7 @@ from dataclasses import dataclass, field
 import torch
 import torch.nn.functional as F
 
-from . import packing, stats
+from . import linear, packing, rotary, sampling, stats
 from .config import QuantConfig
 from .gptq_ref import SweepResult, factor_hessian, gptq_sweep
 from .qronos_ref import qronos_quantize
@@ -107,6 +114,67 @@ class DecoderBlock(torch.nn.Module):
         x = x + self.o_proj(a.transpose(1, 2).reshape(b, s, c.heads * hd))
         h = self.post_attention_layernorm(x)
         return x + self.down_proj(F.silu(self.gate_proj(h)) * self.up_proj(h))
+
+    def decode(self, x, cache: "KVCache", plan: rotary.RotaryPlan):
+        """``forward`` for x [B, S, hidden] that follows the positions already
+        in ``cache``, whose keys and values it extends."""
+        c = self.cfg
+        b, s, _ = x.shape
+        hd = c.hidden // c.heads
+        start, end = cache.length, cache.length + s
+        if end > cache.k.shape[2]:
+            raise ValueError(f"the cache holds {cache.k.shape[2]} positions, {end} are needed")
+        h = self.input_layernorm(x)
+        q = self.q_proj(h).view(b, s, c.heads, hd).transpose(1, 2)
+        k = self.k_proj(h).view(b, s, c.kv_heads, hd).transpose(1, 2)
+        v = self.v_proj(h).view(b, s, c.kv_heads, hd).transpose(1, 2)
+        positions = torch.arange(start, end, device=x.device)
+        q, _ = rotary.apply_rotary(q, k, positions, plan, out=(q, cache.k[:, :, start:end]))
+        cache.v[:, :, start:end] = v
+        cache.length = end
+        rep = c.heads // c.kv_heads
+        k = cache.k[:, :, :end].repeat_interleave(rep, dim=1)
+        v = cache.v[:, :, :end].repeat_interleave(rep, dim=1)
+        mask = None
+        if s > 1:  # position start + i sees the keys up to itself
+            mask = positions[:, None] >= torch.arange(end, device=x.device)[None]
+        a = F.scaled_dot_product_attention(q, k, v, attn_mask=mask)
+        x = x + self.o_proj(a.transpose(1, 2).reshape(b, s, c.heads * hd))
+        h = self.post_attention_layernorm(x)
+        return x + self.down_proj(F.silu(self.gate_proj(h)) * self.up_proj(h))
+
+
+@dataclass
+class KVCache:
+    """Keys (turned by their positions) and values of one block."""
+    k: torch.Tensor   # [B, kv_heads, capacity, head_dim]
+    v: torch.Tensor
+    length: int = 0   # positions held
+
+    @staticmethod
+    def empty(cfg: BlockConfig, batch: int, capacity: int, dtype, device="cuda") -> "KVCache":
+        shape = (batch, cfg.kv_heads, capacity, cfg.hidden // cfg.heads)
+        return KVCache(torch.empty(shape, dtype=dtype, device=device),
+                       torch.empty(shape, dtype=dtype, device=device))
+
+
+def attach_packed(blocks: list[DecoderBlock], checkpoint_dir: str) -> None:
+    """Replace the linears of ``blocks`` by :class:`linear.QuantLinear` on the
+    packed weights of ``checkpoint_dir`` (the ``layer{i}.pt`` files that
+    :func:`quantize_stack` wrote).  The blocks then run, but can no longer be
+    quantized: their float weights are gone."""
+    for i, blk in enumerate(blocks):
+        path = os.path.join(checkpoint_dir, f"layer{i}.pt")
+        packed = packing.load_layer(path, device="cuda")
+        if set(packed) != set(GROUPS):
+            raise ValueError(f"{path} holds {sorted(packed)}, a block has {sorted(GROUPS)}")
+        for name, p in packed.items():
+            lin = getattr(blk, name)
+            if (p.m, p.n) != (lin.out_features, lin.in_features):
+                raise ValueError(f"{path}: {name} is {p.m} x {p.n}, the block's is "
+                                 f"{lin.out_features} x {lin.in_features}")
+        for name, p in packed.items():
+            setattr(blk, name, linear.QuantLinear(p))
 
 
 def synth_stack(n_layers: int, cfg: BlockConfig, seed: int = 0, std: float = 0.02,
@@ -266,6 +334,33 @@ class TinyLM(torch.nn.Module):
         for blk in self.blocks:
             x = blk(x)
         return self.lm_head(self.norm(x))
+
+    @torch.no_grad()
+    def generate(self, ids: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                 min_p=0.0) -> sampling.Sampled:
+        """Continue the prompts ``ids`` [B, T] by one token per column of the
+        uniform numbers ``u`` [B, new], chosen as ``sampling.sample_tokens``
+        does; returns tokens and log-probabilities [B, new].  A row that is
+        left without a token (NaN logits) goes on from token 0."""
+        if ids.dim() != 2 or ids.shape[1] < 1 or u.dim() != 2 or u.shape[0] != ids.shape[0]:
+            raise ValueError(f"ids must be [B, T >= 1] and u [B, new], got {tuple(ids.shape)} and "
+                             f"{tuple(u.shape)}")
+        cfg = self.blocks[0].cfg
+        plan = rotary.rotary_plan(cfg.hidden // cfg.heads, theta=cfg.rope_theta)
+        new = u.shape[1]
+        dtype = self.embed.weight.dtype
+        caches = [KVCache.empty(cfg, ids.shape[0], ids.shape[1] + new, dtype) for _ in self.blocks]
+        tokens = torch.empty((ids.shape[0], new), dtype=torch.int64, device=ids.device)
+        logprobs = torch.empty((ids.shape[0], new), dtype=torch.float32, device=ids.device)
+        for i in range(new):
+            x = self.embed(ids)
+            for blk, cache in zip(self.blocks, caches):
+                x = blk.decode(x, cache, plan)
+            logits = self.lm_head(self.norm(x[:, -1]))
+            got = sampling.sample_tokens(logits, u[:, i], temperature, top_k, top_p, min_p)
+            tokens[:, i], logprobs[:, i] = got
+            ids = got.tokens.clamp_min(0)[:, None]
+        return sampling.Sampled(tokens, logprobs)
 
 
 def stack_forward(blocks, batches):
