@@ -7,7 +7,6 @@ caller's container: numpy in -> numpy out, torch in -> torch (on the device).
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import numpy as np
@@ -53,18 +52,20 @@ def ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.data_ptr())
 
 
+# torch's current stream as a number, without building a Stream object (where
+# this torch has that call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index: int) -> int:
+    """torch's current stream on device ``index``, as the C ABI takes it."""
+    if _raw_stream is not None:
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
+
+
 def stream() -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-_NO_GUARD = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """Context that makes ``device`` current (nothing to do when it is)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _NO_GUARD
-    return torch.cuda.device(device)
+    return ctypes.c_void_p(raw_stream(torch.cuda.current_device()))
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:

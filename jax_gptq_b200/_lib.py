@@ -149,17 +149,22 @@ def exported_symbols() -> list[str]:
     return [n for n in SIGNATURES if getattr(handle, n, None) is not None]
 
 
+def raise_status(status: int):
+    """Raise what a failed call's status means, with the library's message."""
+    msg = lib().gq_last_error().decode(errors="replace")
+    if status == GQ_EINVAL:
+        raise ValueError(msg)
+    if status == GQ_ETIMEOUT:
+        raise DeviceTimeout(status, msg)
+    raise GQError(status, msg)
+
+
 def call(name: str, *args):
     """Call ``name``; raise ``GQError`` (``ValueError`` for GQ_EINVAL) on failure."""
     fn = getattr(lib(), name)
     status = fn(*args)
     if status != GQ_OK:
-        msg = lib().gq_last_error().decode(errors="replace")
-        if status == GQ_EINVAL:
-            raise ValueError(msg)
-        if status == GQ_ETIMEOUT:
-            raise DeviceTimeout(status, msg)
-        raise GQError(status, msg)
+        raise_status(status)
     return status
 
 

@@ -37,7 +37,6 @@ namespace lin {
 constexpr int KC = 128;      // positions per block
 constexpr int ROWS = 16;     // rows per block
 constexpr int WARPS = 8;     // warps of a product CTA, which split K
-constexpr int MAX_NT = 4;    // 8-column tiles of x per CTA
 
 // ---------------------------------------------------------------- layout
 
@@ -72,7 +71,10 @@ __global__ void layout_codes_kernel(const uint32_t* __restrict__ packed, int64_t
 #pragma unroll
         for (int f = 0; f < 8; ++f) {
           const int32_t c = km[f];
-          if (c >= 0) out |= stream_code(src, c, bits) << (4 * (f >> 1) + 16 * (f & 1));
+          if (c >= 0) {
+            const uint32_t v = stream_code(src, c, bits);
+            out |= __funnelshift_l(v, v, 3 + 4 * (f >> 1) + 16 * (f & 1));  // field at bit 3, 7, .. 31, wrapping
+          }
         }
       } else {
         const int jh = wi >> 4, t = (wi >> 2) & 3, jl = (wi >> 1) & 1, h = wi & 1;
@@ -201,20 +203,18 @@ __device__ __forceinline__ uint32_t offset_operand(float o) {
 // The four pairs (code - offset) of 8 positions.  4-bit fields are moved into
 // the mantissa of 16.0, where they count in ones: bits 3-6 of a bf16, bits 6-9
 // of an fp16; 8-bit fields into the mantissa of 2^23 (float) or 1024 (fp16).
+// Field i of a 4-bit word begins at bit 3 + 4 (i / 2) + 16 (i % 2), wrapping, so
+// that the first pair is in place for bf16 and a rotation brings the others.
 template <int WIDTH, bool BF16>
 __device__ __forceinline__ void decode8(const uint32_t* w, uint32_t off, uint32_t (&v)[4]) {
   if constexpr (WIDTH == 4) {
     const uint32_t x = w[0];
-    if constexpr (BF16) {
-      v[0] = ((x << 3) & 0x00780078u) | 0x41804180u;
-      v[1] = ((x >> 1) & 0x00780078u) | 0x41804180u;
-      v[2] = ((x >> 5) & 0x00780078u) | 0x41804180u;
-      v[3] = ((x >> 9) & 0x00780078u) | 0x41804180u;
-    } else {
-      v[0] = ((x << 6) & 0x03c003c0u) | 0x4c004c00u;
-      v[1] = ((x << 2) & 0x03c003c0u) | 0x4c004c00u;
-      v[2] = ((x >> 2) & 0x03c003c0u) | 0x4c004c00u;
-      v[3] = ((x >> 6) & 0x03c003c0u) | 0x4c004c00u;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      if constexpr (BF16)
+        v[p] = (__funnelshift_r(x, x, 4 * p) & 0x00780078u) | 0x41804180u;
+      else
+        v[p] = (__funnelshift_r(x, x, (4 * p + 29) & 31) & 0x03c003c0u) | 0x4c004c00u;
     }
 #pragma unroll
     for (int p = 0; p < 4; ++p) v[p] = sub2<BF16>(v[p], off);
@@ -253,6 +253,15 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Weights are read once: they pass L1 by, where x stays.
+__device__ __forceinline__ uint4 load_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
 struct Args {
   const uint4* qw;
   const float2* params;
@@ -273,14 +282,14 @@ __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 // One CTA: 16 rows, up to 8 NT columns; its warps take contiguous shares of K
 // and their sums are added in warp order.
 template <int WIDTH, typename T, int NT, int G>
-__global__ void __launch_bounds__(32 * WARPS) few_kernel(Args a, bool dependent) {
+__global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2) few_kernel(Args a, bool dependent) {
   constexpr bool BF16 = !std::is_same<T, __half>::value;
   constexpr int SPLIT = std::is_same<T, float>::value ? 3 : 1;
   constexpr int TOK = 8 * NT / SPLIT;  // whole tokens per CTA
   constexpr int JG = G / 32;           // 32-position steps per granule
   constexpr int GPC = KC / G;          // granules per block
   constexpr int LPR = WIDTH / 4;       // 16-byte loads per lane, row and block
-  constexpr int DEPTH = 4;             // blocks in flight per warp
+  constexpr int DEPTH = 3;             // blocks in flight per warp
   __shared__ float red[WARPS][8 * NT][ROWS + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -297,20 +306,20 @@ __global__ void __launch_bounds__(32 * WARPS) few_kernel(Args a, bool dependent)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int l = 0; l < LPR; ++l) d[h][l] = __ldg(b + (g + 8 * h) * (4 * LPR) + l * 4 + t);
+      for (int l = 0; l < LPR; ++l) d[h][l] = load_stream(b + (g + 8 * h) * (4 * LPR) + l * 4 + t);
   };
 #pragma unroll
   for (int s = 0; s < DEPTH; ++s)
     if (c0 + s < c1) fetch(c0 + s, q[s]);
   if (dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
 
+  // a lane without a column reads the first one: columns do not mix
   const uint16_t* xr[NT];
-  bool have[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     const int col = col0 + 8 * i + g;
-    have[i] = 8 * i + g < TOK * SPLIT && col < a.cols;
-    xr[i] = a.x + (have[i] ? (int64_t)col * a.ldx : 0) + 8 * t;
+    xr[i] = a.x + (int64_t)(8 * i + g < TOK * SPLIT && col < a.cols ? col : col0) * a.ldx +
+            (int64_t)c0 * KC + 8 * t;
   }
   float acc[NT][4];
 #pragma unroll
@@ -318,6 +327,17 @@ __global__ void __launch_bounds__(32 * WARPS) few_kernel(Args a, bool dependent)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
 
+  const float2* pc = prow + (int64_t)c0 * (GPC * ROWS) + g;
+  float2 pv[DEPTH][GPC][2];
+  auto fetch_p = [&](float2 (&d)[GPC][2]) {
+#pragma unroll
+    for (int gr = 0; gr < GPC; ++gr) {
+      d[gr][0] = __ldg(pc + gr * ROWS);
+      d[gr][1] = __ldg(pc + gr * ROWS + 8);
+    }
+    pc += GPC * ROWS;
+  };
+  if (c0 < c1) fetch_p(pv[0]);
   for (int cb = c0; cb < c1; cb += DEPTH) {
 #pragma unroll
     for (int s = 0; s < DEPTH; ++s) {
@@ -325,15 +345,15 @@ __global__ void __launch_bounds__(32 * WARPS) few_kernel(Args a, bool dependent)
       if (c >= c1) break;
       uint4 xv[NT][4];
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int i = 0; i < NT; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          xv[i][j] = have[i] ? *reinterpret_cast<const uint4*>(xr[i] + (int64_t)c * KC + 32 * j)
-                             : make_uint4(0, 0, 0, 0);
-      const float2* pc = prow + (int64_t)c * (GPC * ROWS);
+        for (int j = 0; j < 4; ++j) xv[i][j] = *reinterpret_cast<const uint4*>(xr[i] + 32 * j);
+        xr[i] += KC;
+      }
+      if (c + 1 < c1) fetch_p(pv[(s + 1) % DEPTH]);
 #pragma unroll
       for (int gr = 0; gr < GPC; ++gr) {
-        const float2 p0 = __ldg(pc + gr * ROWS + g), p1 = __ldg(pc + gr * ROWS + g + 8);
+        const float2 p0 = pv[s][gr][0], p1 = pv[s][gr][1];
         const uint32_t o0 = offset_operand<WIDTH, BF16>(p0.y);
         const uint32_t o1 = offset_operand<WIDTH, BF16>(p1.y);
         float sum[NT][4];

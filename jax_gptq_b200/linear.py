@@ -128,34 +128,41 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     dt = _DTYPES.get(x.dtype)
     if dt is None:
         raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] != w.n:
-        raise ValueError(f"x must be [..., {w.n}], got {tuple(x.shape)}")
-    if x.device != w.qweight.device:
+    n, m = w.n, w.m
+    if x.dim() < 1 or x.shape[-1] != n:
+        raise ValueError(f"x must be [..., {n}], got {tuple(x.shape)}")
+    dev = x.get_device()
+    if dev < 0 or dev != w.qweight.get_device():
         raise ValueError(f"x is on {x.device}, the weights on {w.qweight.device}")
-    shape = (*x.shape[:-1], w.m)
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= w.n:
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return packed_matmul(x, w, out)
+    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= n:
         x2 = x
     else:
-        x2 = x.reshape(-1, w.n).contiguous()
+        x2 = x.reshape(-1, n).contiguous()
+    tokens, ldx = x2.shape[0], x2.stride(0)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    elif tuple(out.shape) != shape or out.dtype != x.dtype or out.device != x.device or \
-            not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {x.dtype} tensor {shape} on {x.device}")
+        out = x.new_empty((tokens, m) if x2 is x else (*x.shape[:-1], m))
+    elif tuple(out.shape) != (*x.shape[:-1], m) or out.dtype != x.dtype or \
+            out.device != x.device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {x.dtype} tensor {(*x.shape[:-1], m)} on "
+                         f"{x.device}")
     elif A.overlap(out, x2):
         raise ValueError("out shares memory with x")
-    tokens = x2.shape[0]
-    if tokens == 0 or w.m == 0:
+    if tokens == 0 or m == 0:
         return out
-    with A.on_device(x.device):
-        nbytes, ws = 0, None
-        if not (w.direct and dt and x2.data_ptr() % 16 == 0 and x2.stride(0) % 8 == 0):
-            nbytes = _lib.lib().gq_linear_workspace_size(tokens, w.k, dt)
-            ws = A.workspace(nbytes)
-        _lib.call("gq_linear", w.qweight.data_ptr(), w.params.data_ptr(), w.kmap.data_ptr(), w.m,
-                  w.n, w.k, w.bits, w.granule, int(w.direct), x2.data_ptr(), dt, tokens,
-                  x2.stride(0), out.data_ptr(), w.m, None if ws is None else ws.data_ptr(), nbytes,
-                  A.stream())
+    lib = _lib.lib()
+    xp, wp, nbytes = x2.data_ptr(), None, 0
+    if not (w.direct and dt and xp % 16 == 0 and ldx % 8 == 0):  # x is first put in order
+        nbytes = lib.gq_linear_workspace_size(tokens, w.k, dt)
+        ws = A.workspace(nbytes)
+        wp = ws.data_ptr()
+    status = lib.gq_linear(w.qweight.data_ptr(), w.params.data_ptr(), w.kmap.data_ptr(), m, n, w.k,
+                           w.bits, w.granule, w.direct, xp, dt, tokens, ldx, out.data_ptr(), m, wp,
+                           nbytes, A.raw_stream(dev))
+    if status:
+        _lib.raise_status(status)
     return out
 
 

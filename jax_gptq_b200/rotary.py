@@ -19,6 +19,8 @@ from . import _arrays as A
 from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_POSITIONS = (torch.int64, torch.int32)
+_STRIDES = ctypes.c_int64 * 12
 _PI = Fraction("3.14159265358979323846264338327950288419716939937510")
 
 
@@ -147,18 +149,23 @@ def _heads(name: str, x: torch.Tensor, plan: RotaryPlan) -> torch.Tensor:
     return x if x.stride(3) == 1 else x.contiguous()
 
 
-def _result(name: str, x: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
-    if out is None:
-        return torch.empty_like(x)
-    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or \
-            (out.numel() and out.stride(3) != 1):
-        raise ValueError(f"out of {name} must be like it, with contiguous components")
-    if out.numel() > 1 and not A.distinct_elements(out):
-        raise ValueError(f"out of {name} has elements that share memory")
-    same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-    if not same and A.overlap(out, x):
-        raise ValueError(f"out of {name} partly shares memory with it")
-    return out
+def _results(q, k, out):
+    oq, ok = out
+    if oq is None or (ok is None) != (k is None):
+        raise ValueError("out must be a pair like (q, k)")
+    pairs = [("q", q, oq)] + ([] if k is None else [("k", k, ok)])
+    for name, x, o in pairs:
+        if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device or \
+                (o.numel() and o.stride(3) != 1):
+            raise ValueError(f"out of {name} must be like it, with contiguous components")
+        if not A.distinct_elements(o):
+            raise ValueError(f"out of {name} has elements that share memory")
+        same = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
+        if not same and A.overlap(o, x):
+            raise ValueError(f"out of {name} partly shares memory with it")
+    if k is not None and (A.overlap(oq, ok) or A.overlap(oq, k) or A.overlap(ok, q)):
+        raise ValueError("out of q and k share memory with each other or the other input")
+    return oq, ok
 
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
@@ -181,38 +188,44 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         if k.dtype != q.dtype or k.device != q.device:
             raise ValueError("q and k must have one type and device")
         k = _heads("k", k, plan)
-        hk = k.shape[1]
-        if k.shape[0] != b or k.shape[2] != s:
+        kb, hk, ks, _ = k.shape
+        if kb != b or ks != s:
             raise ValueError(f"q and k must have one batch and length, got {tuple(q.shape)} and "
                              f"{tuple(k.shape)}")
-    if positions.dtype not in (torch.int64, torch.int32) or \
-            tuple(positions.shape) not in ((s,), (b, s)):
+    pshape = tuple(positions.shape)
+    if positions.dtype not in _POSITIONS or (pshape != (s,) and pshape != (b, s)):
         raise ValueError(f"positions must be int64 or int32 [{s}] or [{b}, {s}], got "
-                         f"{positions.dtype} {tuple(positions.shape)}")
-    if not q.is_cuda or positions.device != q.device or plan.turns.device != q.device:
+                         f"{positions.dtype} {pshape}")
+    dev = q.get_device()
+    if dev < 0 or positions.get_device() != dev or plan.turns.get_device() != dev:
         raise ValueError(f"q, positions and the plan must be on one CUDA device, got {q.device}, "
                          f"{positions.device} and {plan.turns.device}")
-    if positions.numel() > 1 and positions.stride(-1) != 1:
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return apply_rotary(q, k, positions, plan, out, transpose)
+    if not positions.is_contiguous() and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    oq, ok = (None, None) if out is None else out
-    if out is not None and (oq is None or (ok is None) != (k is None)):
-        raise ValueError("out must be a pair like (q, k)")
-    oq = _result("q", q, oq)
-    if k is not None:
-        ok = _result("k", k, ok)
-        if out is not None and (A.overlap(oq, ok) or A.overlap(oq, k) or A.overlap(ok, q)):
-            raise ValueError("out of q and k share memory with each other or the other input")
-    if oq.numel() + (ok.numel() if k is not None else 0) == 0:
+    if out is None:
+        oq, ok = torch.empty_like(q), None if k is None else torch.empty_like(k)
+    else:
+        oq, ok = _results(q, k, out)
+    if b == 0 or s == 0 or h + hk == 0:
         return oq, ok
-    st = (*q.stride()[:3], *oq.stride()[:3], *(k.stride()[:3] if hk else (0, 0, 0)),
-          *(ok.stride()[:3] if hk else (0, 0, 0)))
-    with A.on_device(q.device):
-        _lib.call("gq_rotary", q.data_ptr(), oq.data_ptr(), h, k.data_ptr() if hk else None,
-                  ok.data_ptr() if hk else None, hk, (ctypes.c_int64 * 12)(*st),
-                  positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0,
-                  int(positions.dtype == torch.int32), plan.turns.data_ptr(), b, s, d,
-                  plan.rotary_dim, int(plan.interleaved), plan.factor, int(transpose), dt,
-                  A.stream())
+    qs, qos = q.stride(), oq.stride()
+    if hk:
+        kst, kos = k.stride(), ok.stride()
+        st = _STRIDES(*qs[:3], *qos[:3], *kst[:3], *kos[:3])
+        kp, kop = k.data_ptr(), ok.data_ptr()
+    else:
+        st = _STRIDES(*qs[:3], *qos[:3])
+        kp = kop = None
+    status = _lib.lib().gq_rotary(
+        q.data_ptr(), oq.data_ptr(), h, kp, kop, hk, st, positions.data_ptr(),
+        positions.stride(0) if len(pshape) == 2 else 0, positions.dtype is torch.int32,
+        plan.turns.data_ptr(), b, s, d, plan.rotary_dim, plan.interleaved, plan.factor, transpose,
+        dt, A.raw_stream(dev))
+    if status:
+        _lib.raise_status(status)
     return oq, ok
 
 

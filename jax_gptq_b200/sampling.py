@@ -23,22 +23,21 @@ class Sampled(NamedTuple):
     logprobs: torch.Tensor  # [rows] float32: log of the token's share of what was kept
 
 
-def _setting(name: str, v, rows: int, device, lo: float, hi: float | None):
+def _setting(name: str, v, rows: int, logits: torch.Tensor, lo: float, hi: float | None):
     """(pointer, kind, value, tensor kept alive) of a setting."""
-    if isinstance(v, torch.Tensor):
-        kind = _KINDS.get(v.dtype)
-        if kind is None:
-            raise ValueError(f"{name} must be float32, float64, int32 or int64, got {v.dtype}")
-        if tuple(v.shape) != (rows,) or v.device != device:
-            raise ValueError(f"{name} must have one value per row ([{rows}] on {device}), got "
-                             f"{tuple(v.shape)} on {v.device}")
-        t = v if v.is_contiguous() else v.contiguous()
-        return t.data_ptr(), kind, 0.0, t
-    f = float(v)
-    if not f >= lo or (hi is not None and f > hi):
-        raise ValueError(f"{name} must be at least {lo}" + (f" and at most {hi}" if hi else "")
-                         + f", got {v}")
-    return None, 0, f, None
+    if not isinstance(v, torch.Tensor):
+        if not v >= lo or (hi is not None and v > hi):
+            raise ValueError(f"{name} must be at least {lo}"
+                             + (f" and at most {hi}" if hi else "") + f", got {v}")
+        return None, 0, v, None
+    kind = _KINDS.get(v.dtype)
+    if kind is None:
+        raise ValueError(f"{name} must be float32, float64, int32 or int64, got {v.dtype}")
+    if v.dim() != 1 or v.shape[0] != rows or v.get_device() != logits.get_device():
+        raise ValueError(f"{name} must have one value per row ([{rows}] on {logits.device}), got "
+                         f"{tuple(v.shape)} on {v.device}")
+    t = v if v.is_contiguous() else v.contiguous()
+    return t.data_ptr(), kind, 0.0, t
 
 
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
@@ -69,19 +68,23 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
         lg = lg.contiguous()
     if u.dtype not in (torch.float32, torch.float64):
         raise ValueError(f"u must be float32 or float64, got {u.dtype}")
-    dev = lg.device
-    up, uk, _, ut = _setting("u", u.reshape(1) if u.dim() == 0 else u, rows, dev, 0.0, None)
-    tp, tk, tv, t0 = _setting("temperature", temperature, rows, dev, 0.0, None)
-    kp, kk, kv, t1 = _setting("top_k", top_k, rows, dev, 0, None)
-    pp, pk, pv, t2 = _setting("top_p", top_p, rows, dev, 0.0, 1.0)
-    mp, mk, mv, t3 = _setting("min_p", min_p, rows, dev, 0.0, 1.0)
-    tokens = torch.empty((rows,), dtype=torch.int64, device=dev)
-    logprobs = torch.empty((rows,), dtype=torch.float32, device=dev)
+    dev = lg.get_device()
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+    up, uk, _, ut = _setting("u", u.reshape(1) if u.dim() == 0 else u, rows, lg, 0.0, None)
+    tp, tk, tv, t0 = _setting("temperature", temperature, rows, lg, 0.0, None)
+    kp, kk, kv, t1 = _setting("top_k", top_k, rows, lg, 0, None)
+    pp, pk, pv, t2 = _setting("top_p", top_p, rows, lg, 0.0, 1.0)
+    mp, mk, mv, t3 = _setting("min_p", min_p, rows, lg, 0.0, 1.0)
+    tokens = lg.new_empty((rows,), dtype=torch.int64)
+    logprobs = lg.new_empty((rows,), dtype=torch.float32)
     if rows:
-        with A.on_device(dev):
-            _lib.call("gq_sample", lg.data_ptr(), dt, rows, vocab, lg.stride(0), up, uk, tp, tk, tv,
-                      kp, kk, kv, pp, pk, pv, mp, mk, mv, tokens.data_ptr(), logprobs.data_ptr(),
-                      A.stream())
+        status = _lib.lib().gq_sample(lg.data_ptr(), dt, rows, vocab, lg.stride(0), up, uk, tp, tk,
+                                      tv, kp, kk, kv, pp, pk, pv, mp, mk, mv, tokens.data_ptr(),
+                                      logprobs.data_ptr(), A.raw_stream(dev))
+        if status:
+            _lib.raise_status(status)
     return Sampled(tokens, logprobs)
 
 
