@@ -11,7 +11,7 @@
 // is off by 0.06.  The wrapped product, a signed fraction of half a turn,
 // becomes a float32 argument of sincospif.
 //
-// Bound: HBM (or, for a few tokens, the launch).  Each block takes TOKENS
+// Bound: HBM (or, for a few tokens, the launch).  Each block takes some
 // positions of one batch entry, works out their cosines and sines once for all
 // heads into shared memory, and reads and writes every head 16 bytes at a time;
 // the first reads are issued before the angles are worked out.
@@ -21,12 +21,12 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace gq {
 namespace rot {
 
-constexpr int THREADS = 256;
-constexpr int AHEAD = 4;  // items a thread has in flight
+constexpr int THREADS = 128;
 
 struct Side {  // one of q and k
   const void* in;
@@ -44,9 +44,11 @@ struct Args {
   const uint64_t* turns;
   int64_t seq;
   int head_dim, half;  // half = rotary_dim / 2
-  int heads;           // of both sides
   int heads_per_block;
+  int q_parts;         // blocks that the heads of q take; those of k follow
   int tokens;          // positions per block
+  int per_head;        // items of a head
+  int half_pad;        // half, to whole 16-byte pieces of floats
   float factor, sign;
 };
 
@@ -67,162 +69,176 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
-// N consecutive components: one access where WIDE (the address is a multiple of
-// its size), else one access each.
-template <typename T, int N, bool WIDE>
-struct alignas(WIDE ? sizeof(T) * N : sizeof(T)) Vec {
-  T e[N];
+// W 32-bit words of components as one access, and as floats.
+template <typename T, int W>
+struct Wide {
+  static constexpr int N = 4 * W / sizeof(T);
+  struct alignas(4 * W) Raw {
+    uint32_t w[W];
+  } raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+  __device__ __forceinline__ void get(float (&f)[N]) const {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const uint32_t w = raw.w[i];
+      if constexpr (sizeof(T) == 4) {
+        f[i] = __uint_as_float(w);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        f[2 * i] = v.x;
+        f[2 * i + 1] = v.y;
+      } else {
+        f[2 * i] = __uint_as_float(w << 16);
+        f[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+      }
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        raw.w[i] = __float_as_uint(f[i]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        raw.w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        raw.w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+  }
 };
-template <typename T, int N, bool WIDE>
-__device__ __forceinline__ void get(Vec<T, N, WIDE>& v, const T* p) {
-  if constexpr (WIDE) {
-    v = *reinterpret_cast<const Vec<T, N, WIDE>*>(p);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v.e[i] = p[i];
-  }
-}
-template <typename T, int N, bool WIDE>
-__device__ __forceinline__ void put(const Vec<T, N, WIDE>& v, T* p) {
-  if constexpr (WIDE) {
-    *reinterpret_cast<Vec<T, N, WIDE>*>(p) = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) p[i] = v.e[i];
-  }
-}
+// One component at a time, for rows that are not made of whole words.
+template <typename T>
+struct Narrow {
+  static constexpr int N = 1;
+  T raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = raw; }
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f<T>(raw); }
+  __device__ __forceinline__ void set(const float (&f)[1]) { raw = from_f<T>(f[0]); }
+};
 
-// One item = V pairs of a head (two vectors in the half layout, one vector of
-// 2 V components in the interleaved one) or a vector (one component where not
-// WIDE) to copy.
-template <typename T, int V, bool INTER, bool WIDE>
+// An item of a head is one piece of each half of N pairs, or in the interleaved
+// layout one piece of N / 2 pairs (two components where Narrow), or one piece to
+// copy.  threadIdx.x is the item inside a head; along y the threads take `hg`
+// heads of q or of k, of `tg` positions at a time.  Many warps with few
+// registers each keep the loads in flight: 4 x 2048 positions of 64 + 8 heads of
+// 128 in bf16 take 52 us (5.8 TB/s of the 302 MB read and written, a plain copy
+// of them 49 us); reading two or four heads ahead in registers took 76 to 94 us.
+template <typename T, typename P, bool INTER>
 __global__ void __launch_bounds__(THREADS) rotary_kernel(Args a) {
-  extern __shared__ float2 cs[];  // [tokens][half]: f cos, f sin
-  constexpr int VI = INTER ? 2 * V : V;
-  constexpr int VC = WIDE ? VI : 1;
-  using Val = Vec<T, VI, WIDE>;
+  constexpr int N = P::N;
+  constexpr bool SPLIT = !INTER || N == 1;  // a pair's components lie in two pieces
+  constexpr int PAIRS = SPLIT ? N : N / 2;
+  extern __shared__ float angles[];  // per position: f cos of every pair, then f sin
   const int64_t s0 = (int64_t)blockIdx.x * a.tokens;
   const int ntok = (int)min((int64_t)a.tokens, a.seq - s0);
   const int64_t b = blockIdx.z;
-  const int h0 = blockIdx.y * a.heads_per_block;
-  const int nh = min(a.heads_per_block, a.heads - h0);
-  const int turn_items = a.half / V;
-  const int copy_items = (a.head_dim - 2 * a.half) / VC;
-  const int per_head = turn_items + copy_items;
-  const int total = ntok * nh * per_head;
+  const int second = blockIdx.y >= a.q_parts;
+  const Side& sd = a.side[second];
+  const int h0 = ((int)blockIdx.y - (second ? a.q_parts : 0)) * a.heads_per_block;
+  const int nh = min(a.heads_per_block, sd.heads - h0);
+  const int half = a.half, half_pad = a.half_pad;
+  const int turn_items = half / PAIRS;
+  const int per_head = a.per_head;
+  const int threads = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
+  const int hg = min((int)blockDim.y, nh), tg = blockDim.y / hg;
+  const int hh = threadIdx.y % hg, tt = threadIdx.y / hg;
 
-  auto where = [&](int item, const T*& in, T*& out, int& tok, int& it) {
-    it = item % per_head;
-    const int rest = item / per_head;
-    tok = rest / nh;
-    int h = h0 + rest % nh;
-    const Side& sd = a.side[h >= a.side[0].heads];
-    if (h >= a.side[0].heads) h -= a.side[0].heads;
-    in = static_cast<const T*>(sd.in) + b * sd.ib + h * sd.ih + (s0 + tok) * sd.is;
-    out = static_cast<T*>(sd.out) + b * sd.ob + h * sd.oh + (s0 + tok) * sd.os;
-  };
-  auto load = [&](int item, Val& x, Val& y) {
-    const T* in;
-    T* out;
-    int tok, it;
-    where(item, in, out, tok, it);
-    if (it >= turn_items) {
-      const T* p = in + 2 * a.half + (it - turn_items) * VC;
-      if constexpr (WIDE) get(x, p);
-      else x.e[0] = *p;
-    } else {
-      get(x, in + it * VI);
-      if constexpr (!INTER) get(y, in + a.half + it * VI);
-    }
-  };
-  auto store = [&](int item, Val& x, Val& y) {
-    const T* in;
-    T* out;
-    int tok, it;
-    where(item, in, out, tok, it);
-    if (it >= turn_items) {
-      T* p = out + 2 * a.half + (it - turn_items) * VC;
-      if constexpr (WIDE) put(x, p);
-      else *p = x.e[0];
-      return;
-    }
-    const float2* c = cs + tok * a.half + it * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      T& p = INTER ? x.e[2 * i] : x.e[i];
-      T& q = INTER ? x.e[2 * i + 1] : y.e[i];
-      const float u = to_f<T>(p), v = to_f<T>(q);
-      const float2 t = c[i];
-      p = from_f<T>(u * t.x - v * t.y);
-      q = from_f<T>(v * t.x + u * t.y);
-    }
-    put(x, out + it * VI);
-    if constexpr (!INTER) put(y, out + a.half + it * VI);
-  };
-
-  Val x[AHEAD], y[AHEAD];
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) {
-    const int item = threadIdx.x + i * THREADS;
-    if (item < total) load(item, x[i], y[i]);
-  }
-  for (int i = threadIdx.x; i < ntok * a.half; i += THREADS) {
-    const int64_t at = b * a.pos_b + s0 + i / a.half;
-    const int64_t pos = a.pos32 ? (int64_t)static_cast<const int32_t*>(a.positions)[at]
-                                : static_cast<const int64_t*>(a.positions)[at];
-    const int64_t frac = (int64_t)((uint64_t)pos * a.turns[i % a.half]);
+  for (int i = tid; i < ntok * half; i += threads) {
+    const int tok = i / half, pair = i - tok * half;
+    const int64_t pi = b * a.pos_b + s0 + tok;
+    const int64_t pos = a.pos32 ? (int64_t)static_cast<const int32_t*>(a.positions)[pi]
+                                : static_cast<const int64_t*>(a.positions)[pi];
+    const int64_t frac = (int64_t)((uint64_t)pos * a.turns[pair]);
     float s, c;
     sincospif((float)frac * 1.0842021724855044e-19f, &s, &c);  // 2^-63
-    cs[i] = make_float2(c * a.factor, s * a.factor * a.sign);
+    angles[tok * 2 * half_pad + pair] = c * a.factor;
+    angles[tok * 2 * half_pad + half_pad + pair] = s * a.factor * a.sign;
   }
   __syncthreads();
-  for (int base = 0; base < total; base += AHEAD * THREADS) {
-    if (base > 0) {
+  if (tt >= tg) return;
+  const int64_t ig = sd.ih * hg, og = sd.oh * hg;
+  for (int it = threadIdx.x; it < per_head; it += blockDim.x) {
+    const bool turn = it < turn_items;
+    // where the item's components begin, and how far its second piece lies
+    const int at = !turn ? 2 * half + (it - turn_items) * N
+                         : (INTER ? it * (SPLIT ? 2 : N) : it * N);
+    const int next = INTER ? 1 : half;
+    for (int tok = tt; tok < ntok; tok += tg) {
+      const T* p = static_cast<const T*>(sd.in) + b * sd.ib + (s0 + tok) * sd.is + (h0 + hh) * sd.ih + at;
+      T* o = static_cast<T*>(sd.out) + b * sd.ob + (s0 + tok) * sd.os + (h0 + hh) * sd.oh + at;
+      float c[PAIRS], s[PAIRS];
+      if (turn) {
+        const float* t = angles + tok * 2 * half_pad + it * PAIRS;
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int item = base + threadIdx.x + i * THREADS;
-        if (item < total) load(item, x[i], y[i]);
+        for (int i = 0; i < PAIRS; ++i) {
+          c[i] = t[i];
+          s[i] = t[half_pad + i];
+        }
       }
-    }
+#pragma unroll 1
+      for (int h = hh; h < nh; h += hg, p += ig, o += og) {
+        P x, y;
+        x.load(p);
+        if (SPLIT && turn) y.load(p + next);
+        if (turn) {
+          float u[N], w[N];
+          x.get(u);
+          if constexpr (SPLIT) y.get(w);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int item = base + threadIdx.x + i * THREADS;
-      if (item < total) store(item, x[i], y[i]);
+          for (int i = 0; i < PAIRS; ++i) {
+            float& e = SPLIT ? u[i] : u[2 * i];
+            float& f = SPLIT ? w[i] : u[2 * i + 1];
+            const float m = e, n = f;
+            e = m * c[i] - n * s[i];
+            f = n * c[i] + m * s[i];
+          }
+          x.set(u);
+          if constexpr (SPLIT) y.set(w);
+        }
+        x.store(o);
+        if (SPLIT && turn) y.store(o + next);
+      }
     }
   }
 }
 
-template <typename T, int V, bool WIDE>
+template <typename T, typename P>
 int run(const Args& a, int64_t batch, bool inter, cudaStream_t st) {
   for (int64_t b0 = 0; b0 < batch; b0 += 65535) {
     Args c = a;
     for (Side& s : c.side) {
+      if (s.heads == 0) continue;
       s.in = static_cast<const T*>(s.in) + b0 * s.ib;
       s.out = static_cast<T*>(s.out) + b0 * s.ob;
     }
     c.positions = static_cast<const char*>(c.positions) + b0 * c.pos_b * (c.pos32 ? 4 : 8);
     const dim3 grid((unsigned)ceil_div(c.seq, c.tokens),
-                    (unsigned)ceil_div(c.heads, c.heads_per_block),
+                    (unsigned)(c.q_parts + ceil_div(c.side[1].heads, c.heads_per_block)),
                     (unsigned)std::min<int64_t>(65535, batch - b0));
-    const size_t smem = (size_t)c.tokens * c.half * sizeof(float2);
+    const size_t smem = (size_t)c.tokens * c.half_pad * 2 * sizeof(float);
+    const int bx = std::min(c.per_head, THREADS);
+    const dim3 block(bx, std::max(1, THREADS / bx));
     if (inter)
-      rotary_kernel<T, V, true, WIDE><<<grid, THREADS, smem, st>>>(c);
+      rotary_kernel<T, P, true><<<grid, block, smem, st>>>(c);
     else
-      rotary_kernel<T, V, false, WIDE><<<grid, THREADS, smem, st>>>(c);
+      rotary_kernel<T, P, false><<<grid, block, smem, st>>>(c);
     GQ_TRY(check_launch("gq_rotary"));
   }
   return GQ_OK;
 }
 
 template <typename T>
-int run_typed(const Args& a, int64_t batch, bool inter, int vec, cudaStream_t st) {
-  constexpr int MAXV = 16 / sizeof(T);
-  // in the interleaved layout an item of V pairs is one access of 2 V components
-  if (vec >= MAXV) {
-    if (inter) return run<T, MAXV / 2, true>(a, batch, inter, st);
-    return run<T, MAXV, true>(a, batch, inter, st);
+int run_typed(const Args& a, int64_t batch, bool inter, int words, cudaStream_t st) {
+  if (words == 4) return run<T, Wide<T, 4>>(a, batch, inter, st);
+  if (words == 2) return run<T, Wide<T, 2>>(a, batch, inter, st);
+  if constexpr (sizeof(T) == 2) {
+    if (words == 1) return run<T, Wide<T, 1>>(a, batch, inter, st);
   }
-  return run<T, 1, false>(a, batch, inter, st);
+  return run<T, Narrow<T>>(a, batch, inter, st);
 }
 
 }  // namespace rot
@@ -246,13 +262,13 @@ extern "C" int gq_rotary(const void* q, void* q_out, int64_t heads, const void* 
   if (batch == 0 || seq == 0 || heads + kv_heads == 0) return GQ_OK;
   GQ_REQUIRE(heads == 0 || (q != nullptr && q_out != nullptr), "gq_rotary: NULL q");
   GQ_REQUIRE(strides != nullptr && positions != nullptr && turns != nullptr, "gq_rotary: NULL input");
-  const size_t size = dtype == 0 ? 4 : 2;
+  const int size = dtype == 0 ? 4 : 2;
   rot::Args a;
-  // 16-byte accesses where every row of both sides starts on such a boundary
-  // and both the turned and the copied part are whole vectors
-  const int maxv = (int)(16 / size);
-  const int64_t unit = interleaved ? rotary_dim : rotary_dim / 2;
-  bool wide = unit % maxv == 0 && (head_dim - rotary_dim) % maxv == 0;
+  // The widest piece, 16 bytes down to one component, that every row of both
+  // sides starts on and that both the turned and the copied part are made of:
+  // all of these are multiples of it, in bytes.
+  uint64_t all = (uint64_t)(interleaved ? rotary_dim : rotary_dim / 2) * size |
+                 (uint64_t)(head_dim - rotary_dim) * size;
   for (int i = 0; i < 2; ++i) {
     const int64_t* s = strides + 6 * i;
     rot::Side& d = a.side[i];
@@ -262,8 +278,8 @@ extern "C" int gq_rotary(const void* q, void* q_out, int64_t heads, const void* 
     d.ob = s[3]; d.oh = s[4]; d.os = s[5];
     d.heads = (int)(i ? kv_heads : heads);
     if (d.heads == 0) continue;
-    for (int e = 0; e < 6; ++e) wide = wide && s[e] % maxv == 0;
-    wide = wide && ((reinterpret_cast<uintptr_t>(d.in) | reinterpret_cast<uintptr_t>(d.out)) & 15) == 0;
+    for (int e = 0; e < 6; ++e) all |= (uint64_t)s[e] * size;
+    all |= reinterpret_cast<uintptr_t>(d.in) | reinterpret_cast<uintptr_t>(d.out);
   }
   a.positions = positions;
   a.pos_b = position_stride;
@@ -272,29 +288,31 @@ extern "C" int gq_rotary(const void* q, void* q_out, int64_t heads, const void* 
   a.seq = seq;
   a.head_dim = head_dim;
   a.half = rotary_dim / 2;
-  a.heads = (int)(heads + kv_heads);
+  a.half_pad = (a.half + 3) & ~3;
   a.factor = factor;
   a.sign = transpose ? -1.f : 1.f;
-  // A block gets about AHEAD items a thread: all heads of as many positions as
-  // that takes (at most 32 KB of angles), or for few positions a part of the heads.
-  const int64_t per_head = wide ? (interleaved ? head_dim / maxv
-                                               : a.half / maxv + (head_dim - rotary_dim) / maxv)
-                                : head_dim - a.half;
-  const int64_t want = rot::THREADS * rot::AHEAD;
-  const int64_t item_tok = per_head * a.heads;
-  int64_t tokens = std::max<int64_t>(1, want / std::max<int64_t>(1, item_tok));
-  tokens = std::min<int64_t>({tokens, seq, std::max<int64_t>(1, 32768 / (a.half * 8))});
-  int64_t hpb = a.heads;
-  if (tokens == 1) hpb = std::max<int64_t>(1, std::min<int64_t>(a.heads, want / per_head));
-  while (hpb > 1 && ceil_div(seq, tokens) * ceil_div(a.heads, hpb) * batch < 148 &&
-         tokens * hpb * per_head > rot::THREADS)
-    hpb = (hpb + 1) / 2;
+  int piece = 16;
+  while (piece > size && all % piece != 0) piece /= 2;
+  const int words = piece > size ? piece / 4 : 0;
+  const int n = words ? piece / size : 1;
+  a.per_head = (interleaved && n > 1 ? rotary_dim / n : a.half / n) + (head_dim - rotary_dim) / n;
+  // A block takes all heads of q or of k, of positions enough for about 8 items
+  // a thread and at most one angle a thread (2 positions of 64 heads of 128: 52
+  // us for 4 x 2048 of them, with 8 positions 57 us); while that leaves SMs
+  // without a block, fewer positions, then fewer heads, down to one item a thread.
+  int64_t hpb = std::max(heads, kv_heads);
+  int64_t tokens = std::max<int64_t>(
+      1, std::min<int64_t>({seq, rot::THREADS / a.half, 8 * rot::THREADS / (hpb * a.per_head)}));
+  auto parts = [&] { return ceil_div(heads, hpb) + ceil_div(kv_heads, hpb); };
+  auto blocks = [&] { return ceil_div(seq, tokens) * parts() * batch; };
+  while (tokens > 1 && blocks() < 4 * sm_count()) tokens = (tokens + 1) / 2;
+  while (hpb > 1 && blocks() < sm_count() && hpb * a.per_head > rot::THREADS) hpb = (hpb + 1) / 2;
   a.tokens = (int)tokens;
   a.heads_per_block = (int)hpb;
-  GQ_REQUIRE(ceil_div(a.heads, hpb) <= 65535, "gq_rotary: too many heads");
+  a.q_parts = (int)ceil_div(heads, hpb);
+  GQ_REQUIRE(parts() <= 65535, "gq_rotary: too many heads");
   cudaStream_t st = as_stream(stream);
-  const int vec = wide ? maxv : 1;
-  if (dtype == 0) return rot::run_typed<float>(a, batch, interleaved != 0, vec, st);
-  if (dtype == 1) return rot::run_typed<__nv_bfloat16>(a, batch, interleaved != 0, vec, st);
-  return rot::run_typed<__half>(a, batch, interleaved != 0, vec, st);
+  if (dtype == 0) return rot::run_typed<float>(a, batch, interleaved != 0, words, st);
+  if (dtype == 1) return rot::run_typed<__nv_bfloat16>(a, batch, interleaved != 0, words, st);
+  return rot::run_typed<__half>(a, batch, interleaved != 0, words, st);
 }
