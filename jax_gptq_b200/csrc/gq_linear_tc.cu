@@ -1,0 +1,679 @@
+// Products with packed weights for many tokens, on the tcgen05 tensor cores.
+//
+// A CTA computes 128 rows of W (the M of the MMA) times TILE columns of x (its
+// N), walking along K in blocks of 128 positions:
+//   D[row, col] += scale[row, granule] * sum_k (code - offset)[row, k] * x[col, k].
+// code - offset is a whole number of at most 8 bits, exact in bf16 and fp16, so
+// each granule is summed in tensor memory from exact products and multiplied by
+// its scale in fp32 registers: nothing about the weights is rounded, as in the
+// few-token form.  A granule's scale is one number per row, which is one number
+// per thread of an epilogue warp (a thread owns a row of tensor memory).
+//
+// Roles (512 threads):
+//   warp 0      TMA producer: x tiles (K-major, 128-byte swizzle), STAGES deep;
+//   warp 1      MMA issuer: A = decoded weights from TENSOR MEMORY, B = x from
+//               shared memory;
+//   warps 4-7   decode: a thread reads its row's codes of a block (64 or 128
+//               bytes, one block ahead), turns them into 128 16-bit numbers and
+//               stores them to one of three tensor-memory buffers (no trip
+//               through shared memory);
+//   warps 8-15  accumulate: granule sums from tensor memory into registers.
+// The tile's columns are two halves with an accumulator each, so that one half
+// is read out while the MMAs fill the other.  Tensor memory: 2 x TILE / 2
+// columns of accumulators and 3 x 64 columns of decoded weights.
+//
+// Where there are fewer tiles than SMs, a cluster of up to 8 CTAs splits K: each
+// leaves its sums in its own shared memory and adds up its share of the columns
+// over the cluster in rank order.  No load uses multicast.
+//
+// Every wait is bounded (gq_set_wait_limit_ns): one that expires makes all roles
+// leave their loops and records GQ_DEVERR_TIMEOUT, read by gq_device_status().
+#include <cuda.h>
+
+#include "gq_linear.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace gq {
+namespace lintc {
+
+using namespace lin;
+
+static __device__ int g_device_status = 0;
+static __device__ uint64_t g_wait_limit_ns = kWaitLimitNs;
+
+int read_status(int reset, int* out) {
+  int v = 0;
+  GQ_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_device_status, sizeof(int)));
+  if (reset) {
+    const int z = 0;
+    GQ_CHECK_CUDA(cudaMemcpyToSymbol(g_device_status, &z, sizeof(int)));
+  }
+  *out = v;
+  return GQ_OK;
+}
+int set_wait_limit(uint64_t ns) {
+  GQ_CHECK_CUDA(cudaMemcpyToSymbol(g_wait_limit_ns, &ns, sizeof(ns)));
+  return GQ_OK;
+}
+
+constexpr int THREADS = 512;
+constexpr int BM = 128;
+constexpr int A_STAGES = 3;
+constexpr int A_COLS = KC / 2;  // tensor-memory columns of one decoded block
+constexpr int TMEM_COLS = 512;
+constexpr int MAX_SMEM = 227 * 1024;
+
+template <int HN>
+struct Cfg {
+  static constexpr int TILE = 2 * HN;              // columns of x per CTA
+  static constexpr int BOX = TILE * 128;           // bytes of 64 positions of the tile
+  static constexpr int STAGE = 2 * BOX;            // one block of 128 positions
+  static constexpr int STAGES = TILE > 192 ? 3 : TILE > 128 ? 4 : 6;
+  static constexpr int PER = HN / 2;               // columns of a half per accumulating thread
+  static constexpr int LD = PER % 32 == 0 ? 32 : PER % 16 == 0 ? 16 : 8;
+  static constexpr int A0 = TILE;                  // first tensor-memory column of the weights
+  static constexpr int SUMS = TILE * BM * 4;       // a tile's sums in shared memory
+  static constexpr int SMEM = (STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS) + 1024 + 256;
+  static_assert(TILE + A_STAGES * A_COLS <= TMEM_COLS, "tensor memory");
+  static_assert(SMEM <= MAX_SMEM, "shared memory");
+};
+
+struct Params {
+  const uint4* qw;
+  const float2* params;
+  int64_t m;
+  int nkc;       // blocks along K
+  int row_blocks;  // blocks of 16 rows
+  int tokens;
+  int mt, nt;    // row tiles, column tiles
+  int split;     // CTAs along K (the cluster size)
+  void* y;
+  int64_t ldy;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait; false when the deadline passed or another role gave up.  The
+// clock is read on every 16th try only.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 15) != 15) continue;
+    if (*abort_flag) return false;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) {
+      t0 = now;
+    } else if (now - t0 > g_wait_limit_ns) {
+      *abort_flag = 1;
+      atomicExch(&g_device_status, GQ_DEVERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+// The same for a whole warp, which stays converged: one lane polls.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity,
+                                               volatile int* abort_flag) {
+  int ok = 0;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag);
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+// Waits, within the limit, for what this thread itself has in flight, whether
+// or not the roles have given up.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i) {
+    if ((i & 15) != 15) continue;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    else if (now - t0 > g_wait_limit_ns) return;
+  }
+}
+__device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* bar, void* dst, int x,
+                                            int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// K-major SW128 descriptor: 8-row groups of 1024 bytes.
+__device__ __forceinline__ uint64_t make_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 |
+         2ull << 61;
+}
+__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                     uint32_t accum) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accum));
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(addr));
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t out;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+  return out;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+
+template <int WIDTH, typename T, int HN, int G>
+__global__ void __launch_bounds__(THREADS, 1)
+many_kernel(const __grid_constant__ CUtensorMap map_x, Params p) {
+  using C = Cfg<HN>;
+  constexpr bool BF16 = !std::is_same<T, __half>::value;
+  constexpr int SPLIT = std::is_same<T, float>::value ? 3 : 1;
+  constexpr int GPC = KC / G;            // granules per block
+  constexpr int TOK = C::TILE / SPLIT;   // tokens per tile
+  constexpr uint32_t IDESC = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) |
+                             ((uint32_t)(HN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  __shared__ uint64_t x_full[C::STAGES], x_empty[C::STAGES], a_full[A_STAGES], a_empty[A_STAGES];
+  __shared__ uint64_t t_full[2], t_empty[2], done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&x_full[s], 1);
+      mbar_init(&x_empty[s], 1);
+    }
+    for (int s = 0; s < A_STAGES; ++s) {
+      mbar_init(&a_full[s], 4);
+      mbar_init(&a_empty[s], 1);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(&t_full[h], 1);
+      mbar_init(&t_empty[h], 8);
+    }
+    mbar_init(&done, 1);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_slot)),
+                 "r"(TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  // this CTA's tiles (one, where a cluster splits K) and its blocks of K
+  const int rank = p.split > 1 ? (int)(blockIdx.x % p.split) : 0;
+  const int first_tile = p.split > 1 ? (int)(blockIdx.x / p.split) : (int)blockIdx.x;
+  const int step = p.split > 1 ? p.mt * p.nt : (int)gridDim.x;
+  const int num_tiles = p.mt * p.nt;
+  const int c0 = (int)((int64_t)p.nkc * rank / p.split), c1 = (int)((int64_t)p.nkc * (rank + 1) / p.split);
+
+  // Registers: 512 threads start with 128 each; warps 0-3 keep 56, the decoders
+  // 96, the accumulating warps take 176: 128 * (56 + 96) + 256 * 176 = 64512.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0 && lane == 0) {
+      int s = 0, loads = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = first_tile; ok && t < num_tiles; t += step) {
+        const int col = (t / p.mt) * (TOK * SPLIT);
+        for (int c = c0; c < c1; ++c) {
+          if (!(ok = mbar_wait(&x_empty[s], phase ^ 1, abort_flag))) break;
+          mbar_expect_tx(&x_full[s], C::STAGE);
+          uint8_t* dst = smem + s * C::STAGE;
+          tma_load_2d(&map_x, &x_full[s], dst, c * KC, col);
+          tma_load_2d(&map_x, &x_full[s], dst + C::BOX, c * KC + 64, col);
+          ++loads;
+          if (++s == C::STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // the MMAs have let go of every stage: no arrival is still on its way
+      for (int i = 0; ok && i < C::STAGES; ++i) {
+        ok = mbar_wait(&x_empty[s], phase ^ 1, abort_flag);
+        if (++s == C::STAGES) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok)  // given up: the loads issued so far still land before the block ends
+        for (int i = 0; i < C::STAGES; ++i) {
+          const int issued = loads / C::STAGES + (i < loads % C::STAGES);
+          if (issued > 0) mbar_drain(&x_full[i], (issued - 1) & 1);
+        }
+    } else if (warp == 1 && lane == 0) {
+      int s = 0, as = 0;
+      uint32_t phase = 0, aphase = 0, tphase = 0;
+      bool ok = true;
+      for (int t = first_tile; ok && t < num_tiles; t += step) {
+        for (int c = c0; ok && c < c1; ++c) {
+          if (!mbar_wait(&x_full[s], phase, abort_flag) || !mbar_wait(&a_full[as], aphase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t b_base = smem_u32(smem + s * C::STAGE);
+          const uint32_t a_base = tmem + C::A0 + as * A_COLS;
+#pragma unroll
+          for (int gr = 0; gr < GPC; ++gr) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (ok && !mbar_wait(&t_empty[h], tphase ^ 1, abort_flag)) ok = false;
+              if (!ok) break;
+              fence_after();
+#pragma unroll
+              for (int i = 0; i < G / 16; ++i) {
+                const int kk = gr * (G / 16) + i;
+                umma(tmem + h * HN, a_base + kk * 8,
+                     make_desc(b_base + (kk / 4) * C::BOX + h * HN * 128 + (kk % 4) * 32), IDESC,
+                     i > 0);
+              }
+              umma_commit(&t_full[h]);
+            }
+            tphase ^= 1;
+          }
+          umma_commit(&x_empty[s]);
+          umma_commit(&a_empty[as]);
+          if (++s == C::STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
+          if (++as == A_STAGES) {
+            as = 0;
+            aphase ^= 1;
+          }
+        }
+      }
+      umma_commit(&done);  // whatever was issued is over before the block ends
+      mbar_drain(&done, 0);
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    constexpr int LPR = WIDTH;  // 16-byte loads per row and block: 4 or 8
+    const int q4 = warp & 3;
+    const int rt = q4 * 32 + lane;  // row of the tile
+    const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+    int as = 0;
+    uint32_t aphase = 0;
+    bool ok = true;
+    for (int t = first_tile; ok && t < num_tiles; t += step) {
+      const int row = (t % p.mt) * BM + rt;
+      const int rb = min(row >> 4, p.row_blocks - 1);  // rows past the last block repeat it, unused
+      const uint4* qp = p.qw + ((int64_t)rb * p.nkc + c0) * (ROWS * LPR) + (row & 15) * LPR;
+      const float2* pp = p.params + ((int64_t)rb * p.nkc + c0) * (GPC * ROWS) + (row & 15);
+      uint4 q[LPR];
+      float off[GPC];
+#pragma unroll
+      for (int i = 0; i < LPR; ++i) q[i] = __ldg(qp + i);
+#pragma unroll
+      for (int i = 0; i < GPC; ++i) off[i] = __ldg(&pp[i * ROWS].y);
+      for (int c = c0; c < c1; ++c) {
+        if (!(ok = mbar_wait_warp(&a_empty[as], aphase ^ 1, abort_flag))) break;
+        fence_after();
+        uint4 cur[LPR];
+        float coff[GPC];
+#pragma unroll
+        for (int i = 0; i < LPR; ++i) cur[i] = q[i];
+#pragma unroll
+        for (int i = 0; i < GPC; ++i) coff[i] = off[i];
+        if (c + 1 < c1) {
+          qp += ROWS * LPR;
+          pp += GPC * ROWS;
+#pragma unroll
+          for (int i = 0; i < LPR; ++i) q[i] = __ldg(qp + i);
+#pragma unroll
+          for (int i = 0; i < GPC; ++i) off[i] = __ldg(&pp[i * ROWS].y);
+        }
+        const uint32_t dst = tmem + lanes + C::A0 + as * A_COLS;
+#pragma unroll
+        for (int jh = 0; jh < 2; ++jh) {
+          uint32_t r[32];
+#pragma unroll
+          for (int jl = 0; jl < 2; ++jl) {
+            const int j = 2 * jh + jl;
+            const uint32_t o = offset_operand<WIDTH, BF16>(coff[j * 32 / G]);
+#pragma unroll
+            for (int tq = 0; tq < 4; ++tq) {
+              uint32_t w[2], v[4];
+              if constexpr (WIDTH == 4) {
+                w[0] = j == 0 ? cur[tq].x : j == 1 ? cur[tq].y : j == 2 ? cur[tq].z : cur[tq].w;
+              } else {
+                w[0] = jl == 0 ? cur[jh * 4 + tq].x : cur[jh * 4 + tq].z;
+                w[1] = jl == 0 ? cur[jh * 4 + tq].y : cur[jh * 4 + tq].w;
+              }
+              decode8<WIDTH, BF16>(w, o, v);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) r[16 * jl + 4 * tq + e] = v[e];
+            }
+          }
+          tmem_st32(dst + 32 * jh, r);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&a_full[as]);
+        if (++as == A_STAGES) {
+          as = 0;
+          aphase ^= 1;
+        }
+      }
+    }
+    for (int i = 0; ok && i < A_STAGES; ++i) {  // as for the x stages
+      ok = mbar_wait_warp(&a_empty[as], aphase ^ 1, abort_flag);
+      if (++as == A_STAGES) {
+        as = 0;
+        aphase ^= 1;
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    const int q4 = warp & 3, part = (warp - 8) >> 2;  // part: which columns of each half
+    const int rt = q4 * 32 + lane;
+    const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+    uint32_t tphase = 0;
+    bool ok = true;
+    for (int t = first_tile; ok && t < num_tiles; t += step) {
+      const int row = (t % p.mt) * BM + rt;
+      const int rb = min(row >> 4, p.row_blocks - 1);
+      const float2* pp = p.params + ((int64_t)rb * p.nkc + c0) * (GPC * ROWS) + (row & 15);
+      float acc[2][C::PER];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < C::PER; ++i) acc[h][i] = 0.f;
+      const int granules = (c1 - c0) * GPC;
+      float scale = granules > 0 ? __ldg(&pp->x) : 0.f;
+      for (int gr = 0; gr < granules; ++gr) {
+        pp += ROWS;
+        const float next = gr + 1 < granules ? __ldg(&pp->x) : 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (ok) ok = mbar_wait_warp(&t_full[h], tphase, abort_flag);
+          if (!ok) break;
+          fence_after();
+#pragma unroll
+          for (int i = 0; i < C::PER; i += C::LD) {
+            uint32_t r[C::LD];
+            tmem_ld(tmem + lanes + h * HN + part * C::PER + i, r);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (i + C::LD >= C::PER) {  // the half is read: the MMAs may refill it
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&t_empty[h]);
+            }
+#pragma unroll
+            for (int e = 0; e < C::LD; ++e)
+              acc[h][i + e] = fmaf(scale, __uint_as_float(r[e]), acc[h][i + e]);
+          }
+        }
+        if (!ok) break;
+        tphase ^= 1;
+        scale = next;
+      }
+      if (!ok) break;
+      const int tok0 = (t / p.mt) * TOK;
+      if (p.split == 1) {
+        T* y = static_cast<T*>(p.y) + row;
+        if (row < p.m) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < C::PER; i += SPLIT) {
+              const int tok = tok0 + (h * HN + part * C::PER + i) / SPLIT;
+              float v = acc[h][i];
+              if constexpr (SPLIT == 3) v = acc[h][i + 2] + acc[h][i + 1] + v;  // small terms first
+              if (tok < p.tokens) store_out(y + (int64_t)tok * p.ldy, v);
+            }
+        }
+      } else {
+        // every MMA and load of this CTA is done: its shared memory is free
+        float* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < C::PER; ++i) sums[(h * HN + part * C::PER + i) * BM + rt] = acc[h][i];
+      }
+    }
+  }
+
+  fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(TMEM_COLS));
+  }
+  if (p.split > 1) {
+    cluster_sync();  // every CTA's sums are in its shared memory
+    const int row0 = (first_tile % p.mt) * BM, tok0 = (first_tile / p.mt) * TOK;
+    const int ntok = min(TOK, p.tokens - tok0);
+    const uint32_t base = smem_u32(smem);
+    const int r = threadIdx.x % BM;
+    if (row0 + r < p.m) {
+      for (int tk = rank * (THREADS / BM) + (int)threadIdx.x / BM; tk < ntok;
+           tk += p.split * (THREADS / BM)) {
+        float v = 0.f;
+#pragma unroll
+        for (int sp = SPLIT - 1; sp >= 0; --sp) {
+          float part = 0.f;
+          for (int c = 0; c < p.split; ++c)
+            part += ld_cluster(peer_addr(base + ((tk * SPLIT + sp) * BM + r) * 4, c));
+          v += part;
+        }
+        store_out(static_cast<T*>(p.y) + (int64_t)(tok0 + tk) * p.ldy + row0 + r, v);
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(ptr);
+  }();
+  return fn;
+}
+
+template <int WIDTH, typename T, int HN, int G>
+int launch(const CUtensorMap& map, const Params& p, cudaStream_t st) {
+  using C = Cfg<HN>;
+  auto kernel = many_kernel<WIDTH, T, HN, G>;
+  static std::atomic<uint64_t> ready{0};  // devices on which the attribute is set
+  int dev = 0;
+  GQ_CHECK_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev > 63 || !(ready.load(std::memory_order_acquire) & bit)) {
+    GQ_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    ready.fetch_or(bit, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  const int tiles = p.mt * p.nt;
+  cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : std::min(tiles, sm_count())));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)p.split, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(GQ_ECUDA, "gq_linear: %s", cudaGetErrorString(e));
+  }
+  return check_launch("gq_linear many-token product");
+}
+
+template <int WIDTH, typename T, int HN>
+int run_tile(const uint16_t* x, int64_t ldx, int64_t k, int granule, Params p, cudaStream_t st) {
+  constexpr int SPLIT = std::is_same<T, float>::value ? 3 : 1;
+  constexpr int TOK = Cfg<HN>::TILE / SPLIT;
+  const int64_t cols = (int64_t)p.tokens * SPLIT;
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(GQ_ECUDA, "cuTensorMapEncodeTiled is unavailable");
+  CUtensorMap map;
+  cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)cols};
+  cuuint64_t strides[1] = {(cuuint64_t)(ldx * 2)};
+  cuuint32_t box[2] = {64, (cuuint32_t)Cfg<HN>::TILE};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r =
+      fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t*>(x), dims, strides, box,
+         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(GQ_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  p.mt = (int)ceil_div(p.m, BM);
+  p.nt = (int)ceil_div(p.tokens, TOK);
+  const int64_t tiles = (int64_t)p.mt * p.nt;
+  GQ_REQUIRE(tiles < (1ll << 31), "gq_linear: too many tiles");
+  // split K over a cluster while that fills idle SMs and leaves 4 blocks each
+  p.split = 1;
+  while (p.split < 8 && tiles * p.split * 2 <= sm_count() && p.nkc >= p.split * 2 * 4) p.split *= 2;
+  if (granule == 128) return launch<WIDTH, T, HN, 128>(map, p, st);
+  if (granule == 64) return launch<WIDTH, T, HN, 64>(map, p, st);
+  return launch<WIDTH, T, HN, 32>(map, p, st);
+}
+
+template <int WIDTH, typename T>
+int run_typed(const uint16_t* x, int64_t ldx, int64_t k, int granule, const Params& p,
+              cudaStream_t st) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (p.tokens <= 32) return run_tile<WIDTH, T, 48>(x, ldx, k, granule, p, st);
+    return run_tile<WIDTH, T, 96>(x, ldx, k, granule, p, st);
+  } else {
+    if (p.tokens <= 32) return run_tile<WIDTH, T, 16>(x, ldx, k, granule, p, st);
+    if (p.tokens <= 64) return run_tile<WIDTH, T, 32>(x, ldx, k, granule, p, st);
+    if (p.tokens <= 128) return run_tile<WIDTH, T, 64>(x, ldx, k, granule, p, st);
+    return run_tile<WIDTH, T, 128>(x, ldx, k, granule, p, st);
+  }
+}
+
+}  // namespace lintc
+
+namespace lin {
+
+int run_many(const uint32_t* qw, const float* params, int64_t m, int64_t k, int bits, int granule,
+             const uint16_t* x, int64_t ldx, int dtype, int64_t tokens, void* y, int64_t ldy,
+             cudaStream_t st) {
+  lintc::Params p = {};
+  p.qw = reinterpret_cast<const uint4*>(qw);
+  p.params = reinterpret_cast<const float2*>(params);
+  p.m = m;
+  p.nkc = (int)(k / KC);
+  p.row_blocks = (int)ceil_div(m, ROWS);
+  p.tokens = (int)tokens;
+  p.y = y;
+  p.ldy = ldy;
+  if (bits <= 4) {
+    if (dtype == 0) return lintc::run_typed<4, float>(x, ldx, k, granule, p, st);
+    if (dtype == 1) return lintc::run_typed<4, __nv_bfloat16>(x, ldx, k, granule, p, st);
+    return lintc::run_typed<4, __half>(x, ldx, k, granule, p, st);
+  }
+  if (dtype == 0) return lintc::run_typed<8, float>(x, ldx, k, granule, p, st);
+  if (dtype == 1) return lintc::run_typed<8, __nv_bfloat16>(x, ldx, k, granule, p, st);
+  return lintc::run_typed<8, __half>(x, ldx, k, granule, p, st);
+}
+
+}  // namespace lin
+}  // namespace gq

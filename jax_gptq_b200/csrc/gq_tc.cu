@@ -937,6 +937,11 @@ int set_wait_limit(uint64_t ns);
 int launch_expire_test(int* observed, cudaStream_t st);
 }
 
+namespace lintc {
+int read_status(int reset, int* out);
+int set_wait_limit(uint64_t ns);
+}
+
 }  // namespace gq
 
 extern "C" {
@@ -964,7 +969,8 @@ int gq_set_wait_limit_ns(uint64_t ns) {
   GQ_REQUIRE(ns >= 1000000ull && ns <= 60000000000ull,
              "gq_set_wait_limit_ns: %llu ns is outside [1 ms, 60 s]", (unsigned long long)ns);
   GQ_TRY(gq::tc::set_wait_limit(ns));
-  return gq::tc32::set_wait_limit(ns);
+  GQ_TRY(gq::tc32::set_wait_limit(ns));
+  return gq::lintc::set_wait_limit(ns);
 }
 
 int gq_test_expire_wait(int unit, int* observed, void* stream) {
@@ -997,7 +1003,9 @@ int gq_device_status(int* status_out, int reset, void* stream) {
   }
   int v32 = 0;
   GQ_TRY(gq::tc32::read_status(reset, &v32));
-  *status_out = v ? v : v32;
+  int vlin = 0;
+  GQ_TRY(gq::lintc::read_status(reset, &vlin));
+  *status_out = v ? v : v32 ? v32 : vlin;
   return GQ_OK;
 }
 
