@@ -14,6 +14,9 @@
 // field i of word j of lane t of its quad, so one 16-byte load per lane and
 // row holds the lane's share of 128 positions, and the other operand's
 // matching 8 values (positions 32 j + 8 t ..) are 16 contiguous bytes of x.
+// The 16-byte pieces of a row are permuted with the row (piece_at), so that
+// eight threads that read one piece of eight rows from shared memory meet eight
+// different bank groups.
 // params[(rb * K / G + granule) * 16 + r] = {scale, offset}: offset = zero -
 // qmin is a whole number (the quantizers round it), so the weight is
 // (code - offset) * scale.
@@ -52,9 +55,9 @@ __global__ void layout_codes_kernel(const uint32_t* __restrict__ packed, int64_t
   constexpr int WPR = KC * WIDTH / 32;  // words per block row: 16 or 32
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total_words;
        i += (int64_t)gridDim.x * blockDim.x) {
-    const int wi = (int)(i % WPR);
     const int64_t rest = i / WPR;
     const int r = (int)(rest % ROWS);
+    const int wi = ((int)(i % WPR) & 3) | piece_at<WIDTH>((int)(i % WPR) >> 2, r) << 2;
     const int64_t blk = rest / ROWS;
     const int64_t kc = blk % nkc, row = (blk / nkc) * ROWS + r;
     uint32_t out = 0;
@@ -231,7 +234,8 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2) few_kernel(Args a
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int l = 0; l < LPR; ++l) d[h][l] = load_stream(b + (g + 8 * h) * (4 * LPR) + l * 4 + t);
+      for (int l = 0; l < LPR; ++l)
+        d[h][l] = load_stream(b + (g + 8 * h) * (4 * LPR) + piece_at<WIDTH>(l * 4 + t, g));
   };
 #pragma unroll
   for (int s = 0; s < DEPTH; ++s)

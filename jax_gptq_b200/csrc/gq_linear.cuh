@@ -15,6 +15,14 @@ namespace lin {
 constexpr int KC = 128;      // positions per block
 constexpr int ROWS = 16;     // rows per block
 
+// Place of 16-byte piece `i` in row r of a block (its own inverse): the row's 4
+// (8) pieces are exchanged so that pieces i of 8 consecutive rows cover 128
+// different bytes modulo 128.
+template <int WIDTH>
+__host__ __device__ __forceinline__ int piece_at(int i, int r) {
+  return WIDTH == 4 ? i ^ ((r >> 1) & 3) : i ^ (r & 7);
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
   uint32_t d;

@@ -9,18 +9,22 @@
 // few-token form.  A granule's scale is one number per row, which is one number
 // per thread of an epilogue warp (a thread owns a row of tensor memory).
 //
-// Roles (512 threads):
-//   warp 0      TMA producer: x tiles (K-major, 128-byte swizzle), STAGES deep;
+// Roles (640 threads):
+//   warp 0      TMA producer: x tiles of 128 positions (K-major, 128-byte
+//               swizzle), three in flight;
 //   warp 1      MMA issuer: A = decoded weights from TENSOR MEMORY, B = x from
-//               shared memory;
-//   warps 4-7   decode: a thread reads its row's codes of a block (64 or 128
-//               bytes, one block ahead), turns them into 128 16-bit numbers and
-//               stores them to one of three tensor-memory buffers (no trip
-//               through shared memory);
-//   warps 8-15  accumulate: granule sums from tensor memory into registers.
-// The tile's columns are two halves with an accumulator each, so that one half
-// is read out while the MMAs fill the other.  Tensor memory: 2 x TILE / 2
-// columns of accumulators and 3 x 64 columns of decoded weights.
+//               shared memory.  The whole warp walks the loop, so that addresses
+//               and descriptors stay in uniform registers, and one lane is
+//               elected to issue;
+//   warp 2      copies a block's codes and scales to shared memory;
+//   warps 4-11  decode: a thread turns its row's codes of a block into 128 16-bit
+//               numbers and stores them to one of three tensor-memory buffers.
+//               The two groups of four warps take alternate blocks: one group
+//               alone needed 2200 cycles a block, twice what the MMAs need;
+//   warps 12-19 accumulate: granule sums from tensor memory into registers.
+// There are two accumulators.  Tiles of up to 128 columns use them in turn, one
+// granule each; wider tiles are two halves with one each, so that one half is
+// read out while the MMAs fill the other.
 //
 // Where there are fewer tiles than SMs, a cluster of up to 8 CTAs splits K: each
 // leaves its sums in its own shared memory and adds up its share of the columns
@@ -58,26 +62,32 @@ int set_wait_limit(uint64_t ns) {
   return GQ_OK;
 }
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 640;
 constexpr int BM = 128;
-constexpr int A_STAGES = 3;
+constexpr int STAGES = 3;       // blocks of x and of decoded weights
 constexpr int A_COLS = KC / 2;  // tensor-memory columns of one decoded block
 constexpr int TMEM_COLS = 512;
 constexpr int MAX_SMEM = 227 * 1024;
 
-template <int HN>
+// N: columns of an MMA, PARTS: MMAs side by side (1 or 2).
+template <int WIDTH, int N, int PARTS, int G>
 struct Cfg {
-  static constexpr int TILE = 2 * HN;              // columns of x per CTA
+  static constexpr int TILE = N * PARTS;           // columns of x per CTA
   static constexpr int BOX = TILE * 128;           // bytes of 64 positions of the tile
-  static constexpr int STAGE = 2 * BOX;            // one block of 128 positions
-  static constexpr int STAGES = TILE > 192 ? 3 : TILE > 128 ? 4 : 6;
-  static constexpr int PER = HN / 2;               // columns of a half per accumulating thread
-  static constexpr int LD = PER % 32 == 0 ? 32 : PER % 16 == 0 ? 16 : 8;
-  static constexpr int A0 = TILE;                  // first tensor-memory column of the weights
+  static constexpr int XSTAGE = 2 * BOX;           // a block of 128 positions
+  static constexpr int CODES = BM * KC * WIDTH / 8;        // a block's codes of 128 rows
+  static constexpr int SCALES = BM * (KC / G) * 8;         // and its scales and offsets
+  static constexpr int WSTAGE = CODES + SCALES;
+  static constexpr int WSTAGES = TILE > 192 ? (G < 128 ? 2 : 3) : 4;
+  static constexpr int PER = N / 2;                // columns of a part per accumulating thread
+  static constexpr int LD = PER % 16 == 0 ? 16 : 8;
+  static constexpr int A0 = 2 * N;                 // first tensor-memory column of the weights
   static constexpr int SUMS = TILE * BM * 4;       // a tile's sums in shared memory
-  static constexpr int SMEM = (STAGES * STAGE > SUMS ? STAGES * STAGE : SUMS) + 1024 + 256;
-  static_assert(TILE + A_STAGES * A_COLS <= TMEM_COLS, "tensor memory");
-  static_assert(SMEM <= MAX_SMEM, "shared memory");
+  static constexpr int W0 = STAGES * XSTAGE;       // where the weights' stages begin
+  static constexpr int USED = W0 + WSTAGES * WSTAGE;
+  static constexpr int SMEM = (USED > SUMS ? USED : SUMS) + 1024;
+  static_assert(2 * N + STAGES * A_COLS <= TMEM_COLS, "tensor memory");
+  static_assert(SMEM + 1024 <= MAX_SMEM, "shared memory");
 };
 
 struct Params {
@@ -161,6 +171,19 @@ __device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* ba
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst, int x,
+                                            int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+  return e != 0;
+}
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -185,29 +208,13 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
           smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31, %32};" ::"r"(addr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16};" ::"r"(addr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
-      "r"(r[30]), "r"(r[31])
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
 }
 __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
@@ -239,20 +246,24 @@ __device__ __forceinline__ void cluster_sync() {
                    : "memory");
 }
 
-template <int WIDTH, typename T, int HN, int G>
+template <int WIDTH, typename T, int N, int PARTS, int G>
 __global__ void __launch_bounds__(THREADS, 1)
-many_kernel(const __grid_constant__ CUtensorMap map_x, Params p) {
-  using C = Cfg<HN>;
+many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+            const __grid_constant__ CUtensorMap map_s, Params p) {
+  using C = Cfg<WIDTH, N, PARTS, G>;
   constexpr bool BF16 = !std::is_same<T, __half>::value;
   constexpr int SPLIT = std::is_same<T, float>::value ? 3 : 1;
   constexpr int GPC = KC / G;            // granules per block
   constexpr int TOK = C::TILE / SPLIT;   // tokens per tile
   constexpr uint32_t IDESC = (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) |
-                             ((uint32_t)(HN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+                             ((uint32_t)(N >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  __shared__ uint64_t x_full[C::STAGES], x_empty[C::STAGES], a_full[A_STAGES], a_empty[A_STAGES];
+  // full: x has landed and the four decoding warps have stored the weights;
+  // empty: the block's MMAs are over
+  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ uint64_t w_full[C::WSTAGES], w_empty[C::WSTAGES];
   __shared__ uint64_t t_full[2], t_empty[2], done;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
@@ -260,13 +271,13 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, Params p) {
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&x_full[s], 1);
-      mbar_init(&x_empty[s], 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1 + 4);
+      mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < A_STAGES; ++s) {
-      mbar_init(&a_full[s], 4);
-      mbar_init(&a_empty[s], 1);
+    for (int s = 0; s < C::WSTAGES; ++s) {
+      mbar_init(&w_full[s], 1);
+      mbar_init(&w_empty[s], 4);  // the decoding warps of a block
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(&t_full[h], 1);
@@ -295,201 +306,204 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, Params p) {
   const int num_tiles = p.mt * p.nt;
   const int c0 = (int)((int64_t)p.nkc * rank / p.split), c1 = (int)((int64_t)p.nkc * (rank + 1) / p.split);
 
-  // Registers: 512 threads start with 128 each; warps 0-3 keep 56, the decoders
-  // 96, the accumulating warps take 176: 128 * (56 + 96) + 256 * 176 = 64512.
+  // Registers: 640 threads start with 96 each; warps 0-3 keep 40, the decoders
+  // 56, the accumulating warps take 160: 128 * 40 + 256 * 56 + 256 * 160 = 60416.
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0 && lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 1) {
+      int s = 0;
+      uint32_t phase = 0, u = 0;  // u: parts of granules issued; accumulator u & 1
+      bool ok = true;
+      for (int t = first_tile; ok && t < num_tiles; t += step) {
+        for (int c = c0; ok && c < c1; ++c) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase, abort_flag));
+          if (!ok) break;
+          const uint32_t b_base = smem_u32(smem) + s * C::XSTAGE;
+          const uint32_t a_base = tmem + C::A0 + s * A_COLS;
+#pragma unroll
+          for (int gr = 0; gr < GPC; ++gr) {
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) {
+              const uint32_t buf = PARTS == 2 ? h : u & 1;
+              ok = ok && __all_sync(0xffffffffu, mbar_wait(&t_empty[buf], ((u >> 1) & 1) ^ 1, abort_flag));
+              ++u;
+              if (!ok) break;
+              fence_after();
+              if (elect_one()) {
+#pragma unroll
+                for (int i = 0; i < G / 16; ++i) {
+                  const int kk = gr * (G / 16) + i;
+                  umma(tmem + buf * N, a_base + kk * 8,
+                       make_desc(b_base + (kk / 4) * C::BOX + h * N * 128 + (kk % 4) * 32), IDESC, i > 0);
+                }
+                umma_commit(&t_full[buf]);
+                if (gr == GPC - 1 && h == PARTS - 1) umma_commit(&empty[s]);
+              }
+              __syncwarp();
+            }
+          }
+          if (++s == STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (elect_one()) {
+        umma_commit(&done);  // whatever was issued is over before the block ends
+        mbar_drain(&done, 0);
+      }
+    } else if (warp == 0 || warp == 2) {
+      // copies by tensor map: x; codes and scales of 8 blocks of 16 rows (rows
+      // past the last block read as zeros)
+      const int stages = warp == 0 ? STAGES : C::WSTAGES;
+      uint64_t* fb = warp == 0 ? full : w_full;
+      uint64_t* eb = warp == 0 ? empty : w_empty;
       int s = 0, loads = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int t = first_tile; ok && t < num_tiles; t += step) {
-        const int col = (t / p.mt) * (TOK * SPLIT);
+        const int col = (t / p.mt) * (TOK * SPLIT), rb0 = (t % p.mt) * (BM / ROWS);
         for (int c = c0; c < c1; ++c) {
-          if (!(ok = mbar_wait(&x_empty[s], phase ^ 1, abort_flag))) break;
-          mbar_expect_tx(&x_full[s], C::STAGE);
-          uint8_t* dst = smem + s * C::STAGE;
-          tma_load_2d(&map_x, &x_full[s], dst, c * KC, col);
-          tma_load_2d(&map_x, &x_full[s], dst + C::BOX, c * KC + 64, col);
+          if (!(ok = mbar_wait_warp(&eb[s], phase ^ 1, abort_flag))) break;
+          if (lane == 0) {
+            if (warp == 0) {
+              uint8_t* dst = smem + s * C::XSTAGE;
+              mbar_expect_tx(&fb[s], C::XSTAGE);
+              tma_load_2d(&map_x, &fb[s], dst, c * KC, col);
+              tma_load_2d(&map_x, &fb[s], dst + C::BOX, c * KC + 64, col);
+            } else {
+              uint8_t* dst = smem + C::W0 + s * C::WSTAGE;
+              mbar_expect_tx(&fb[s], C::WSTAGE);
+              tma_load_3d(&map_w, &fb[s], dst, 0, c, rb0);
+              tma_load_3d(&map_s, &fb[s], dst + C::CODES, 0, c, rb0);
+            }
+          }
           ++loads;
-          if (++s == C::STAGES) {
+          if (++s == stages) {
             s = 0;
             phase ^= 1;
           }
         }
       }
-      // the MMAs have let go of every stage: no arrival is still on its way
-      for (int i = 0; ok && i < C::STAGES; ++i) {
-        ok = mbar_wait(&x_empty[s], phase ^ 1, abort_flag);
-        if (++s == C::STAGES) {
+      // Every stage was let go of: no arrival is still on its way.  Where the
+      // roles gave up, the copies issued so far still land before the block ends
+      // (x's barrier may lack the decoders' arrivals; then the limit ends the wait).
+      for (int i = 0; ok && i < stages; ++i) {
+        ok = mbar_wait_warp(&eb[s], phase ^ 1, abort_flag);
+        if (++s == stages) {
           s = 0;
           phase ^= 1;
         }
       }
-      if (!ok)  // given up: the loads issued so far still land before the block ends
-        for (int i = 0; i < C::STAGES; ++i) {
-          const int issued = loads / C::STAGES + (i < loads % C::STAGES);
-          if (issued > 0) mbar_drain(&x_full[i], (issued - 1) & 1);
+      if (!ok && lane == 0)
+        for (int i = 0; i < stages; ++i) {
+          const int issued = loads / stages + (i < loads % stages);
+          if (issued > 0) mbar_drain(&fb[i], (issued - 1) & 1);
         }
-    } else if (warp == 1 && lane == 0) {
-      int s = 0, as = 0;
-      uint32_t phase = 0, aphase = 0, tphase = 0;
-      bool ok = true;
-      for (int t = first_tile; ok && t < num_tiles; t += step) {
-        for (int c = c0; ok && c < c1; ++c) {
-          if (!mbar_wait(&x_full[s], phase, abort_flag) || !mbar_wait(&a_full[as], aphase, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const uint32_t b_base = smem_u32(smem + s * C::STAGE);
-          const uint32_t a_base = tmem + C::A0 + as * A_COLS;
-#pragma unroll
-          for (int gr = 0; gr < GPC; ++gr) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (ok && !mbar_wait(&t_empty[h], tphase ^ 1, abort_flag)) ok = false;
-              if (!ok) break;
-              fence_after();
-#pragma unroll
-              for (int i = 0; i < G / 16; ++i) {
-                const int kk = gr * (G / 16) + i;
-                umma(tmem + h * HN, a_base + kk * 8,
-                     make_desc(b_base + (kk / 4) * C::BOX + h * HN * 128 + (kk % 4) * 32), IDESC,
-                     i > 0);
-              }
-              umma_commit(&t_full[h]);
-            }
-            tphase ^= 1;
-          }
-          umma_commit(&x_empty[s]);
-          umma_commit(&a_empty[as]);
-          if (++s == C::STAGES) {
-            s = 0;
-            phase ^= 1;
-          }
-          if (++as == A_STAGES) {
-            as = 0;
-            aphase ^= 1;
-          }
-        }
-      }
-      umma_commit(&done);  // whatever was issued is over before the block ends
-      mbar_drain(&done, 0);
     }
     __syncwarp();
-  } else if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     constexpr int LPR = WIDTH;  // 16-byte loads per row and block: 4 or 8
     const int q4 = warp & 3;
     const int rt = q4 * 32 + lane;  // row of the tile
     const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
-    int as = 0;
-    uint32_t aphase = 0;
+    // n: blocks so far; this group takes every second one
+    const int mine = (warp >> 2) & 1;
+    uint32_t n = 0;
     bool ok = true;
     for (int t = first_tile; ok && t < num_tiles; t += step) {
-      const int row = (t % p.mt) * BM + rt;
-      const int rb = min(row >> 4, p.row_blocks - 1);  // rows past the last block repeat it, unused
-      const uint4* qp = p.qw + ((int64_t)rb * p.nkc + c0) * (ROWS * LPR) + (row & 15) * LPR;
-      const float2* pp = p.params + ((int64_t)rb * p.nkc + c0) * (GPC * ROWS) + (row & 15);
-      uint4 q[LPR];
-      float off[GPC];
-#pragma unroll
-      for (int i = 0; i < LPR; ++i) q[i] = __ldg(qp + i);
-#pragma unroll
-      for (int i = 0; i < GPC; ++i) off[i] = __ldg(&pp[i * ROWS].y);
-      for (int c = c0; c < c1; ++c) {
-        if (!(ok = mbar_wait_warp(&a_empty[as], aphase ^ 1, abort_flag))) break;
-        fence_after();
+      for (int c = c0; c < c1; ++c, ++n) {
+        if ((n & 1) != mine) continue;
+        const int ws = n % C::WSTAGES, as = n % STAGES;
+        if (!(ok = mbar_wait_warp(&w_full[ws], (n / C::WSTAGES) & 1, abort_flag))) break;
+        const uint8_t* stage = smem + C::W0 + ws * C::WSTAGE;
+        const uint4* codes = reinterpret_cast<const uint4*>(stage) + rt * LPR;
+        const float2* sc = reinterpret_cast<const float2*>(stage + C::CODES) +
+                           (rt >> 4) * (GPC * ROWS) + (rt & 15);
         uint4 cur[LPR];
         float coff[GPC];
 #pragma unroll
-        for (int i = 0; i < LPR; ++i) cur[i] = q[i];
+        for (int i = 0; i < LPR; ++i) cur[i] = codes[piece_at<WIDTH>(i, rt)];
 #pragma unroll
-        for (int i = 0; i < GPC; ++i) coff[i] = off[i];
-        if (c + 1 < c1) {
-          qp += ROWS * LPR;
-          pp += GPC * ROWS;
-#pragma unroll
-          for (int i = 0; i < LPR; ++i) q[i] = __ldg(qp + i);
-#pragma unroll
-          for (int i = 0; i < GPC; ++i) off[i] = __ldg(&pp[i * ROWS].y);
-        }
+        for (int i = 0; i < GPC; ++i) coff[i] = sc[i * ROWS].y;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w_empty[ws]);
+        if (!(ok = mbar_wait_warp(&empty[as], ((n / STAGES) & 1) ^ 1, abort_flag))) break;
+        fence_after();
         const uint32_t dst = tmem + lanes + C::A0 + as * A_COLS;
 #pragma unroll
-        for (int jh = 0; jh < 2; ++jh) {
-          uint32_t r[32];
+        for (int j = 0; j < 4; ++j) {
+          uint32_t r[16];
+          const uint32_t o = offset_operand<WIDTH, BF16>(coff[j * 32 / G]);
 #pragma unroll
-          for (int jl = 0; jl < 2; ++jl) {
-            const int j = 2 * jh + jl;
-            const uint32_t o = offset_operand<WIDTH, BF16>(coff[j * 32 / G]);
-#pragma unroll
-            for (int tq = 0; tq < 4; ++tq) {
-              uint32_t w[2], v[4];
-              if constexpr (WIDTH == 4) {
-                w[0] = j == 0 ? cur[tq].x : j == 1 ? cur[tq].y : j == 2 ? cur[tq].z : cur[tq].w;
-              } else {
-                w[0] = jl == 0 ? cur[jh * 4 + tq].x : cur[jh * 4 + tq].z;
-                w[1] = jl == 0 ? cur[jh * 4 + tq].y : cur[jh * 4 + tq].w;
-              }
-              decode8<WIDTH, BF16>(w, o, v);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) r[16 * jl + 4 * tq + e] = v[e];
+          for (int tq = 0; tq < 4; ++tq) {
+            uint32_t w[2], v[4];
+            if constexpr (WIDTH == 4) {
+              w[0] = j == 0 ? cur[tq].x : j == 1 ? cur[tq].y : j == 2 ? cur[tq].z : cur[tq].w;
+            } else {
+              const uint4& q = cur[(j >> 1) * 4 + tq];
+              w[0] = (j & 1) == 0 ? q.x : q.z;
+              w[1] = (j & 1) == 0 ? q.y : q.w;
             }
+            decode8<WIDTH, BF16>(w, o, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[4 * tq + e] = v[e];
           }
-          tmem_st32(dst + 32 * jh, r);
+          tmem_st16(dst + 16 * j, r);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&a_full[as]);
-        if (++as == A_STAGES) {
-          as = 0;
-          aphase ^= 1;
-        }
-      }
-    }
-    for (int i = 0; ok && i < A_STAGES; ++i) {  // as for the x stages
-      ok = mbar_wait_warp(&a_empty[as], aphase ^ 1, abort_flag);
-      if (++as == A_STAGES) {
-        as = 0;
-        aphase ^= 1;
+        if (lane == 0) mbar_arrive(&full[as]);
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-    const int q4 = warp & 3, part = (warp - 8) >> 2;  // part: which columns of each half
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    const int q4 = warp & 3, part = (warp - 12) >> 2;  // part: which columns of each half
     const int rt = q4 * 32 + lane;
     const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
-    uint32_t tphase = 0;
+    uint32_t u = 0;
     bool ok = true;
     for (int t = first_tile; ok && t < num_tiles; t += step) {
       const int row = (t % p.mt) * BM + rt;
-      const int rb = min(row >> 4, p.row_blocks - 1);
-      const float2* pp = p.params + ((int64_t)rb * p.nkc + c0) * (GPC * ROWS) + (row & 15);
-      float acc[2][C::PER];
+      // the scales of a row, AHEAD granules before they are needed
+      constexpr int AHEAD = GPC == 1 ? 2 : 4;
+      const float2* pp = p.params + ((int64_t)min(row >> 4, p.row_blocks - 1) * p.nkc + c0) * (GPC * ROWS) + (row & 15);
+      float acc[PARTS][C::PER];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < PARTS; ++h)
 #pragma unroll
         for (int i = 0; i < C::PER; ++i) acc[h][i] = 0.f;
       const int granules = (c1 - c0) * GPC;
-      float scale = granules > 0 ? __ldg(&pp->x) : 0.f;
-      for (int gr = 0; gr < granules; ++gr) {
-        pp += ROWS;
-        const float next = gr + 1 < granules ? __ldg(&pp->x) : 0.f;
+      float ahead[AHEAD];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (ok) ok = mbar_wait_warp(&t_full[h], tphase, abort_flag);
+      for (int i = 0; i < AHEAD; ++i) {
+        ahead[i] = i < granules ? __ldg(&pp->x) : 0.f;
+        pp += ROWS;
+      }
+      for (int gr = 0; gr < granules; ++gr) {
+        const float scale = ahead[0];
+#pragma unroll
+        for (int i = 0; i + 1 < AHEAD; ++i) ahead[i] = ahead[i + 1];
+        if (gr + AHEAD < granules) ahead[AHEAD - 1] = __ldg(&pp->x);
+        pp += ROWS;
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h) {
+          const uint32_t buf = PARTS == 2 ? h : u & 1;
+          if (ok) ok = mbar_wait_warp(&t_full[buf], (u >> 1) & 1, abort_flag);
+          ++u;
           if (!ok) break;
           fence_after();
 #pragma unroll
           for (int i = 0; i < C::PER; i += C::LD) {
             uint32_t r[C::LD];
-            tmem_ld(tmem + lanes + h * HN + part * C::PER + i, r);
+            tmem_ld(tmem + lanes + buf * N + part * C::PER + i, r);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (i + C::LD >= C::PER) {  // the half is read: the MMAs may refill it
+            if (i + C::LD >= C::PER) {  // the part is read: the MMAs may refill it
               fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(&t_empty[h]);
+              if (lane == 0) mbar_arrive(&t_empty[buf]);
             }
 #pragma unroll
             for (int e = 0; e < C::LD; ++e)
@@ -497,8 +511,6 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, Params p) {
           }
         }
         if (!ok) break;
-        tphase ^= 1;
-        scale = next;
       }
       if (!ok) break;
       const int tok0 = (t / p.mt) * TOK;
@@ -506,10 +518,10 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, Params p) {
         T* y = static_cast<T*>(p.y) + row;
         if (row < p.m) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < PARTS; ++h)
 #pragma unroll
             for (int i = 0; i < C::PER; i += SPLIT) {
-              const int tok = tok0 + (h * HN + part * C::PER + i) / SPLIT;
+              const int tok = tok0 + (h * N + part * C::PER + i) / SPLIT;
               float v = acc[h][i];
               if constexpr (SPLIT == 3) v = acc[h][i + 2] + acc[h][i + 1] + v;  // small terms first
               if (tok < p.tokens) store_out(y + (int64_t)tok * p.ldy, v);
@@ -519,9 +531,9 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, Params p) {
         // every MMA and load of this CTA is done: its shared memory is free
         float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < PARTS; ++h)
 #pragma unroll
-          for (int i = 0; i < C::PER; ++i) sums[(h * HN + part * C::PER + i) * BM + rt] = acc[h][i];
+          for (int i = 0; i < C::PER; ++i) sums[(h * N + part * C::PER + i) * BM + rt] = acc[h][i];
       }
     }
   }
@@ -575,10 +587,29 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-template <int WIDTH, typename T, int HN, int G>
-int launch(const CUtensorMap& map, const Params& p, cudaStream_t st) {
-  using C = Cfg<HN>;
-  auto kernel = many_kernel<WIDTH, T, HN, G>;
+// [blocks][along][inner] of `size`-byte elements, read 8 blocks at a time.
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int inner,
+                    int64_t along, int64_t blocks, int size) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(GQ_ECUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)along, (cuuint64_t)blocks};
+  cuuint64_t strides[2] = {(cuuint64_t)inner * size, (cuuint64_t)inner * size * along};
+  cuuint32_t box[3] = {(cuuint32_t)inner, 1, BM / ROWS};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, type, 3, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(GQ_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return GQ_OK;
+}
+
+template <int WIDTH, typename T, int N, int PARTS, int G>
+int launch(const CUtensorMap& map, const CUtensorMap& map_w, const Params& p, cudaStream_t st) {
+  using C = Cfg<WIDTH, N, PARTS, G>;
+  auto kernel = many_kernel<WIDTH, T, N, PARTS, G>;
+  CUtensorMap map_s;  // [row blocks][blocks of K][16 rows x granules of a scale and an offset]
+  GQ_TRY(make_map(&map_s, CU_TENSOR_MAP_DATA_TYPE_INT64, p.params, ROWS * (KC / G), p.nkc,
+                  p.row_blocks, 8));
   static std::atomic<uint64_t> ready{0};  // devices on which the attribute is set
   int dev = 0;
   GQ_CHECK_CUDA(cudaGetDevice(&dev));
@@ -598,7 +629,7 @@ int launch(const CUtensorMap& map, const Params& p, cudaStream_t st) {
   at[0].val.clusterDim = {(unsigned)p.split, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = p.split > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map, map_w, map_s, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(GQ_ECUDA, "gq_linear: %s", cudaGetErrorString(e));
@@ -606,23 +637,26 @@ int launch(const CUtensorMap& map, const Params& p, cudaStream_t st) {
   return check_launch("gq_linear many-token product");
 }
 
-template <int WIDTH, typename T, int HN>
+template <int WIDTH, typename T, int N, int PARTS>
 int run_tile(const uint16_t* x, int64_t ldx, int64_t k, int granule, Params p, cudaStream_t st) {
   constexpr int SPLIT = std::is_same<T, float>::value ? 3 : 1;
-  constexpr int TOK = Cfg<HN>::TILE / SPLIT;
+  constexpr int TOK = (N * PARTS) / SPLIT;
   const int64_t cols = (int64_t)p.tokens * SPLIT;
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(GQ_ECUDA, "cuTensorMapEncodeTiled is unavailable");
   CUtensorMap map;
   cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)cols};
   cuuint64_t strides[1] = {(cuuint64_t)(ldx * 2)};
-  cuuint32_t box[2] = {64, (cuuint32_t)Cfg<HN>::TILE};
+  cuuint32_t box[2] = {64, (cuuint32_t)(N * PARTS)};
   cuuint32_t estr[2] = {1, 1};
   const CUresult r =
       fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t*>(x), dims, strides, box,
          estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(GQ_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  CUtensorMap map_w;  // a block's 16 rows of codes: 256 elements of 4 or 8 bytes
+  GQ_TRY(make_map(&map_w, WIDTH == 4 ? CU_TENSOR_MAP_DATA_TYPE_INT32 : CU_TENSOR_MAP_DATA_TYPE_INT64,
+                  p.qw, 256, p.nkc, p.row_blocks, WIDTH));
   p.mt = (int)ceil_div(p.m, BM);
   p.nt = (int)ceil_div(p.tokens, TOK);
   const int64_t tiles = (int64_t)p.mt * p.nt;
@@ -630,22 +664,23 @@ int run_tile(const uint16_t* x, int64_t ldx, int64_t k, int granule, Params p, c
   // split K over a cluster while that fills idle SMs and leaves 4 blocks each
   p.split = 1;
   while (p.split < 8 && tiles * p.split * 2 <= sm_count() && p.nkc >= p.split * 2 * 4) p.split *= 2;
-  if (granule == 128) return launch<WIDTH, T, HN, 128>(map, p, st);
-  if (granule == 64) return launch<WIDTH, T, HN, 64>(map, p, st);
-  return launch<WIDTH, T, HN, 32>(map, p, st);
+  if (granule == 128) return launch<WIDTH, T, N, PARTS, 128>(map, map_w, p, st);
+  if (granule == 64) return launch<WIDTH, T, N, PARTS, 64>(map, map_w, p, st);
+  return launch<WIDTH, T, N, PARTS, 32>(map, map_w, p, st);
 }
 
 template <int WIDTH, typename T>
 int run_typed(const uint16_t* x, int64_t ldx, int64_t k, int granule, const Params& p,
               cudaStream_t st) {
-  if constexpr (std::is_same<T, float>::value) {
-    if (p.tokens <= 32) return run_tile<WIDTH, T, 48>(x, ldx, k, granule, p, st);
-    return run_tile<WIDTH, T, 96>(x, ldx, k, granule, p, st);
+  if constexpr (std::is_same<T, float>::value) {  // three columns a token
+    if (p.tokens <= 32) return run_tile<WIDTH, T, 96, 1>(x, ldx, k, granule, p, st);
+    return run_tile<WIDTH, T, 96, 2>(x, ldx, k, granule, p, st);
   } else {
-    if (p.tokens <= 32) return run_tile<WIDTH, T, 16>(x, ldx, k, granule, p, st);
-    if (p.tokens <= 64) return run_tile<WIDTH, T, 32>(x, ldx, k, granule, p, st);
-    if (p.tokens <= 128) return run_tile<WIDTH, T, 64>(x, ldx, k, granule, p, st);
-    return run_tile<WIDTH, T, 128>(x, ldx, k, granule, p, st);
+    if (p.tokens <= 32) return run_tile<WIDTH, T, 32, 1>(x, ldx, k, granule, p, st);
+    if (p.tokens <= 64) return run_tile<WIDTH, T, 64, 1>(x, ldx, k, granule, p, st);
+    if (p.tokens <= 128) return run_tile<WIDTH, T, 128, 1>(x, ldx, k, granule, p, st);
+    // 256 columns and the 8-bit codes' stages together exceed shared memory
+    return run_tile<WIDTH, T, WIDTH == 4 ? 128 : 96, 2>(x, ldx, k, granule, p, st);
   }
 }
 
