@@ -21,10 +21,12 @@
 //               numbers and stores them to one of three tensor-memory buffers.
 //               The two groups of four warps take alternate blocks: one group
 //               alone needed 2200 cycles a block, twice what the MMAs need;
-//   warps 12-19 accumulate: granule sums from tensor memory into registers.
+//   warps 12-19 accumulate: granule sums from tensor memory into registers, two
+//               columns a multiply-add (fma.rn.f32x2).
 // There are two accumulators.  Tiles of up to 128 columns use them in turn, one
-// granule each; wider tiles are two halves with one each, so that one half is
-// read out while the MMAs fill the other.
+// granule each, and each group of four accumulating warps takes half the
+// columns; wider tiles are two halves with an accumulator and a group each, so
+// that one half is read out while the MMAs fill the other.
 //
 // Where there are fewer tiles than SMs, a cluster of up to 8 CTAs splits K: each
 // leaves its sums in its own shared memory and adds up its share of the columns
@@ -79,7 +81,7 @@ struct Cfg {
   static constexpr int SCALES = BM * (KC / G) * 8;         // and its scales and offsets
   static constexpr int WSTAGE = CODES + SCALES;
   static constexpr int WSTAGES = TILE > 192 ? (G < 128 ? 2 : 3) : 4;
-  static constexpr int PER = N / 2;                // columns of a part per accumulating thread
+  static constexpr int PER = PARTS == 2 ? N : N / 2;  // columns per accumulating thread
   static constexpr int LD = PER % 16 == 0 ? 16 : 8;
   static constexpr int A0 = 2 * N;                 // first tensor-memory column of the weights
   static constexpr int SUMS = TILE * BM * 4;       // a tile's sums in shared memory
@@ -195,17 +197,19 @@ __device__ __forceinline__ uint64_t make_desc(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 |
          2ull << 61;
 }
-__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                     uint32_t accum) {
+// Executed by the whole warp; the thread with `leader` set issues.
+__device__ __forceinline__ void umma(uint32_t leader, uint32_t d, uint32_t a, uint64_t b,
+                                     uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accum));
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accum), "r"(leader));
 }
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+__device__ __forceinline__ void umma_commit(uint32_t leader, uint64_t* bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          smem_u32(bar))
+      "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(
+          smem_u32(bar)), "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
@@ -230,6 +234,30 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[8]) {
       "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
       : "r"(addr));
+}
+// Waits for this thread's tensor-memory loads; the registers pass through, so
+// that nothing that uses them moves above.
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7])
+               :
+               : "memory");
+}
+// {a0, a1} = scale * {r0, r1} + {a0, a1}
+__device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t r0, uint32_t r1, float scale) {
+  asm("{\n .reg .b64 a, r, s;\n mov.b64 a, {%0, %1};\n mov.b64 r, {%2, %3};\n mov.b64 s, {%4, %4};\n"
+      " fma.rn.f32x2 a, r, s, a;\n mov.b64 {%0, %1}, a;\n}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(__uint_as_float(r0)), "f"(__uint_as_float(r1)), "f"(scale));
 }
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
@@ -281,7 +309,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(&t_full[h], 1);
-      mbar_init(&t_empty[h], 8);
+      mbar_init(&t_empty[h], PARTS == 2 ? 4 : 8);  // the warps that read it
     }
     mbar_init(&done, 1);
     abort_word = 0;
@@ -313,6 +341,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     if (warp == 1) {
       int s = 0;
       uint32_t phase = 0, u = 0;  // u: parts of granules issued; accumulator u & 1
+      const uint32_t leader = elect_one();
       bool ok = true;
       for (int t = first_tile; ok && t < num_tiles; t += step) {
         for (int c = c0; ok && c < c1; ++c) {
@@ -329,16 +358,14 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
               ++u;
               if (!ok) break;
               fence_after();
-              if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < G / 16; ++i) {
-                  const int kk = gr * (G / 16) + i;
-                  umma(tmem + buf * N, a_base + kk * 8,
-                       make_desc(b_base + (kk / 4) * C::BOX + h * N * 128 + (kk % 4) * 32), IDESC, i > 0);
-                }
-                umma_commit(&t_full[buf]);
-                if (gr == GPC - 1 && h == PARTS - 1) umma_commit(&empty[s]);
+              for (int i = 0; i < G / 16; ++i) {
+                const int kk = gr * (G / 16) + i;
+                umma(leader, tmem + buf * N, a_base + kk * 8,
+                     make_desc(b_base + (kk / 4) * C::BOX + h * N * 128 + (kk % 4) * 32), IDESC, i > 0);
               }
+              umma_commit(leader, &t_full[buf]);
+              if (gr == GPC - 1 && h == PARTS - 1) umma_commit(leader, &empty[s]);
               __syncwarp();
             }
           }
@@ -348,10 +375,8 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
           }
         }
       }
-      if (elect_one()) {
-        umma_commit(&done);  // whatever was issued is over before the block ends
-        mbar_drain(&done, 0);
-      }
+      umma_commit(leader, &done);  // whatever was issued is over before the block ends
+      mbar_drain(&done, 0);
     } else if (warp == 0 || warp == 2) {
       // copies by tensor map: x; codes and scales of 8 blocks of 16 rows (rows
       // past the last block read as zeros)
@@ -470,11 +495,9 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       // the scales of a row, AHEAD granules before they are needed
       constexpr int AHEAD = GPC == 1 ? 2 : 4;
       const float2* pp = p.params + ((int64_t)min(row >> 4, p.row_blocks - 1) * p.nkc + c0) * (GPC * ROWS) + (row & 15);
-      float acc[PARTS][C::PER];
+      float acc[C::PER];
 #pragma unroll
-      for (int h = 0; h < PARTS; ++h)
-#pragma unroll
-        for (int i = 0; i < C::PER; ++i) acc[h][i] = 0.f;
+      for (int i = 0; i < C::PER; ++i) acc[i] = 0.f;
       const int granules = (c1 - c0) * GPC;
       float ahead[AHEAD];
 #pragma unroll
@@ -488,52 +511,50 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         for (int i = 0; i + 1 < AHEAD; ++i) ahead[i] = ahead[i + 1];
         if (gr + AHEAD < granules) ahead[AHEAD - 1] = __ldg(&pp->x);
         pp += ROWS;
-#pragma unroll
-        for (int h = 0; h < PARTS; ++h) {
-          const uint32_t buf = PARTS == 2 ? h : u & 1;
-          if (ok) ok = mbar_wait_warp(&t_full[buf], (u >> 1) & 1, abort_flag);
-          ++u;
-          if (!ok) break;
-          fence_after();
-#pragma unroll
-          for (int i = 0; i < C::PER; i += C::LD) {
-            uint32_t r[C::LD];
-            tmem_ld(tmem + lanes + buf * N + part * C::PER + i, r);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (i + C::LD >= C::PER) {  // the part is read: the MMAs may refill it
-              fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&t_empty[buf]);
-            }
-#pragma unroll
-            for (int e = 0; e < C::LD; ++e)
-              acc[h][i + e] = fmaf(scale, __uint_as_float(r[e]), acc[h][i + e]);
-          }
-        }
+        // wide tiles: this group's half of every granule; else every granule's
+        // half of the columns
+        const uint32_t buf = PARTS == 2 ? part : u & 1;
+        ok = mbar_wait_warp(&t_full[buf], PARTS == 2 ? u & 1 : (u >> 1) & 1, abort_flag);
+        ++u;
         if (!ok) break;
+        fence_after();
+        const uint32_t src = tmem + lanes + buf * N + (PARTS == 2 ? 0 : part * C::PER);
+        uint32_t r[2][C::LD];
+        tmem_ld(src, r[0]);
+#pragma unroll
+        for (int i = 0; i < C::PER; i += C::LD) {
+          uint32_t(&v)[C::LD] = r[(i / C::LD) & 1];
+          tmem_wait(v);
+          if (i + C::LD < C::PER) {
+            tmem_ld(src + i + C::LD, r[(i / C::LD + 1) & 1]);
+          } else {  // all is read: the MMAs may refill the accumulator
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&t_empty[buf]);
+          }
+#pragma unroll
+          for (int e = 0; e < C::LD; e += 2) fma2(acc[i + e], acc[i + e + 1], v[e], v[e + 1], scale);
+        }
       }
       if (!ok) break;
       const int tok0 = (t / p.mt) * TOK;
+      const int col0 = part * C::PER;
       if (p.split == 1) {
         T* y = static_cast<T*>(p.y) + row;
         if (row < p.m) {
 #pragma unroll
-          for (int h = 0; h < PARTS; ++h)
-#pragma unroll
-            for (int i = 0; i < C::PER; i += SPLIT) {
-              const int tok = tok0 + (h * N + part * C::PER + i) / SPLIT;
-              float v = acc[h][i];
-              if constexpr (SPLIT == 3) v = acc[h][i + 2] + acc[h][i + 1] + v;  // small terms first
-              if (tok < p.tokens) store_out(y + (int64_t)tok * p.ldy, v);
-            }
+          for (int i = 0; i < C::PER; i += SPLIT) {
+            const int tok = tok0 + (col0 + i) / SPLIT;
+            float v = acc[i];
+            if constexpr (SPLIT == 3) v = acc[i + 2] + acc[i + 1] + v;  // small terms first
+            if (tok < p.tokens) store_out(y + (int64_t)tok * p.ldy, v);
+          }
         }
       } else {
         // every MMA and load of this CTA is done: its shared memory is free
         float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (int h = 0; h < PARTS; ++h)
-#pragma unroll
-          for (int i = 0; i < C::PER; ++i) sums[(h * N + part * C::PER + i) * BM + rt] = acc[h][i];
+        for (int i = 0; i < C::PER; ++i) sums[(col0 + i) * BM + rt] = acc[i];
       }
     }
   }
