@@ -11,22 +11,24 @@
 //
 // Roles (640 threads):
 //   warp 0      TMA producer: x tiles of 128 positions (K-major, 128-byte
-//               swizzle), three in flight;
+//               swizzle), several in flight;
 //   warp 1      MMA issuer: A = decoded weights from TENSOR MEMORY, B = x from
 //               shared memory.  The whole warp walks the loop, so that addresses
 //               and descriptors stay in uniform registers, and one lane is
 //               elected to issue;
 //   warp 2      copies a block's codes and scales to shared memory;
 //   warps 4-11  decode: a thread turns its row's codes of a block into 128 16-bit
-//               numbers and stores them to one of three tensor-memory buffers.
+//               numbers and stores them to one of 2 or 3 tensor-memory buffers.
 //               The two groups of four warps take alternate blocks: one group
 //               alone needed 2200 cycles a block, twice what the MMAs need;
 //   warps 12-19 accumulate: granule sums from tensor memory into registers, two
 //               columns a multiply-add (fma.rn.f32x2).
-// There are two accumulators.  Tiles of up to 128 columns use them in turn, one
-// granule each, and each group of four accumulating warps takes half the
-// columns; wider tiles are two halves with an accumulator and a group each, so
-// that one half is read out while the MMAs fill the other.
+// Three accumulators (two in one form) are used in turn, one for each granule's MMAs over the
+// tile's columns, or over half of them where the tile is wider than 128: filling
+// one (512 cycles for 128 positions of 128 columns) and then reading it out takes
+// about 1600 cycles with the signals in between, so with two the tensor pipe idled
+// half the time.  In wide tiles each group of four accumulating warps has a half
+// of the columns, else half of every granule's.
 //
 // Where there are fewer tiles than SMs, a cluster of up to 8 CTAs splits K: each
 // leaves its sums in its own shared memory and adds up its share of the columns
@@ -66,7 +68,6 @@ int set_wait_limit(uint64_t ns) {
 
 constexpr int THREADS = 640;
 constexpr int BM = 128;
-constexpr int STAGES = 3;       // blocks of x and of decoded weights
 constexpr int A_COLS = KC / 2;  // tensor-memory columns of one decoded block
 constexpr int TMEM_COLS = 512;
 constexpr int MAX_SMEM = 227 * 1024;
@@ -77,18 +78,25 @@ struct Cfg {
   static constexpr int TILE = N * PARTS;           // columns of x per CTA
   static constexpr int BOX = TILE * 128;           // bytes of 64 positions of the tile
   static constexpr int XSTAGE = 2 * BOX;           // a block of 128 positions
+  static constexpr int STAGES = TILE > 128 ? 3 : 4;   // blocks of x
+  // accumulators and decoded blocks: tensor memory has room for 3 of both only
+  // with narrower MMAs; a tile of one part needs the decoded blocks more (128
+  // tokens through 11008 x 4096: 26 us against 30), one of two the accumulators
+  static constexpr int ACCS = N > 96 && PARTS == 1 ? 2 : 3;
+  static constexpr int ASTAGES = N > 96 && PARTS == 2 ? 2 : 3;
   static constexpr int CODES = BM * KC * WIDTH / 8;        // a block's codes of 128 rows
   static constexpr int SCALES = BM * (KC / G) * 8;         // and its scales and offsets
   static constexpr int WSTAGE = CODES + SCALES;
   static constexpr int WSTAGES = TILE > 192 ? (G < 128 ? 2 : 3) : 4;
   static constexpr int PER = PARTS == 2 ? N : N / 2;  // columns per accumulating thread
   static constexpr int LD = PER % 16 == 0 ? 16 : 8;
-  static constexpr int A0 = 2 * N;                 // first tensor-memory column of the weights
+  static constexpr int A0 = ACCS * N;                 // first tensor-memory column of the weights
   static constexpr int SUMS = TILE * BM * 4;       // a tile's sums in shared memory
   static constexpr int W0 = STAGES * XSTAGE;       // where the weights' stages begin
   static constexpr int USED = W0 + WSTAGES * WSTAGE;
   static constexpr int SMEM = (USED > SUMS ? USED : SUMS) + 1024;
-  static_assert(2 * N + STAGES * A_COLS <= TMEM_COLS, "tensor memory");
+  static_assert(ACCS * N + ASTAGES * A_COLS <= TMEM_COLS, "tensor memory");
+  static_assert(SUMS <= W0, "sums only over x");
   static_assert(SMEM + 1024 <= MAX_SMEM, "shared memory");
 };
 
@@ -123,6 +131,17 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// The same without waiting at all (try_wait may hold the thread for a while).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
       " selp.u32 %0, 1, 0, p;\n}"
       : "=r"(ok)
       : "r"(smem_u32(bar)), "r"(parity)
@@ -288,26 +307,28 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  // full: x has landed and the four decoding warps have stored the weights;
-  // empty: the block's MMAs are over
-  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ uint64_t x_full[C::STAGES], x_empty[C::STAGES], a_full[C::ASTAGES], a_empty[C::ASTAGES];
   __shared__ uint64_t w_full[C::WSTAGES], w_empty[C::WSTAGES];
-  __shared__ uint64_t t_full[2], t_empty[2], done;
+  __shared__ uint64_t t_full[C::ACCS], t_empty[C::ACCS], done;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1 + 4);
-      mbar_init(&empty[s], 1);
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&x_full[s], 1);
+      mbar_init(&x_empty[s], 1);
+    }
+    for (int s = 0; s < C::ASTAGES; ++s) {
+      mbar_init(&a_full[s], 4);  // the decoding warps of a block
+      mbar_init(&a_empty[s], 1);
     }
     for (int s = 0; s < C::WSTAGES; ++s) {
       mbar_init(&w_full[s], 1);
       mbar_init(&w_empty[s], 4);  // the decoding warps of a block
     }
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < C::ACCS; ++h) {
       mbar_init(&t_full[h], 1);
       mbar_init(&t_empty[h], PARTS == 2 ? 4 : 8);  // the warps that read it
     }
@@ -339,50 +360,69 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 1) {
-      int s = 0;
-      uint32_t phase = 0, u = 0;  // u: parts of granules issued; accumulator u & 1
+      // Every barrier is looked at once before the MMAs ahead of it are issued, so
+      // that the answer is there when it is needed.
+      int s = 0, as = 0, acc = 0;
+      uint32_t phase = 0, aphase = 0, tphase = 0;
       const uint32_t leader = elect_one();
-      bool ok = true;
-      for (int t = first_tile; ok && t < num_tiles; t += step) {
-        for (int c = c0; ok && c < c1; ++c) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[s], phase, abort_flag));
-          if (!ok) break;
-          const uint32_t b_base = smem_u32(smem) + s * C::XSTAGE;
-          const uint32_t a_base = tmem + C::A0 + s * A_COLS;
+      const int blocks = (c1 - c0) * ((num_tiles - first_tile + step - 1) / step);
+      bool ok = true, x_ready = false, a_ready = false, t_ready = false;
+      for (int n = 0; n < blocks; ++n) {
+        ok = (x_ready || mbar_wait(&x_full[s], phase, abort_flag)) &&
+             (a_ready || mbar_wait(&a_full[as], aphase, abort_flag));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t b_base = smem_u32(smem) + s * C::XSTAGE;
+        const uint32_t a_base = tmem + C::A0 + as * A_COLS;
+        uint64_t* const x_done = &x_empty[s];
+        uint64_t* const a_done = &a_empty[as];
+        if (++s == C::STAGES) {
+          s = 0;
+          phase ^= 1;
+        }
+        if (++as == C::ASTAGES) {
+          as = 0;
+          aphase ^= 1;
+        }
 #pragma unroll
-          for (int gr = 0; gr < GPC; ++gr) {
+        for (int gr = 0; gr < GPC; ++gr) {
 #pragma unroll
-            for (int h = 0; h < PARTS; ++h) {
-              const uint32_t buf = PARTS == 2 ? h : u & 1;
-              ok = ok && __all_sync(0xffffffffu, mbar_wait(&t_empty[buf], ((u >> 1) & 1) ^ 1, abort_flag));
-              ++u;
-              if (!ok) break;
-              fence_after();
-#pragma unroll
-              for (int i = 0; i < G / 16; ++i) {
-                const int kk = gr * (G / 16) + i;
-                umma(leader, tmem + buf * N, a_base + kk * 8,
-                     make_desc(b_base + (kk / 4) * C::BOX + h * N * 128 + (kk % 4) * 32), IDESC, i > 0);
-              }
-              umma_commit(leader, &t_full[buf]);
-              if (gr == GPC - 1 && h == PARTS - 1) umma_commit(leader, &empty[s]);
-              __syncwarp();
+          for (int h = 0; h < PARTS; ++h) {
+            ok = ok && (t_ready || mbar_wait(&t_empty[acc], tphase ^ 1, abort_flag));
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int cur = acc;
+            if (++acc == C::ACCS) {
+              acc = 0;
+              tphase ^= 1;
             }
-          }
-          if (++s == STAGES) {
-            s = 0;
-            phase ^= 1;
+            t_ready = mbar_test(&t_empty[acc], tphase ^ 1);
+            if (gr == GPC - 1 && h == PARTS - 1) {
+              x_ready = mbar_test(&x_full[s], phase);
+              a_ready = mbar_test(&a_full[as], aphase);
+            }
+            fence_after();
+#pragma unroll
+            for (int i = 0; i < G / 16; ++i) {
+              const int kk = gr * (G / 16) + i;
+              umma(leader, tmem + cur * N, a_base + kk * 8,
+                   make_desc(b_base + (kk / 4) * C::BOX + h * N * 128 + (kk % 4) * 32), IDESC, i > 0);
+            }
+            umma_commit(leader, &t_full[cur]);
           }
         }
+        if (!ok) break;
+        umma_commit(leader, a_done);
+        umma_commit(leader, x_done);
       }
       umma_commit(leader, &done);  // whatever was issued is over before the block ends
       mbar_drain(&done, 0);
     } else if (warp == 0 || warp == 2) {
       // copies by tensor map: x; codes and scales of 8 blocks of 16 rows (rows
       // past the last block read as zeros)
-      const int stages = warp == 0 ? STAGES : C::WSTAGES;
-      uint64_t* fb = warp == 0 ? full : w_full;
-      uint64_t* eb = warp == 0 ? empty : w_empty;
+      const int stages = warp == 0 ? C::STAGES : C::WSTAGES;
+      uint64_t* fb = warp == 0 ? x_full : w_full;
+      uint64_t* eb = warp == 0 ? x_empty : w_empty;
       int s = 0, loads = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -411,8 +451,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         }
       }
       // Every stage was let go of: no arrival is still on its way.  Where the
-      // roles gave up, the copies issued so far still land before the block ends
-      // (x's barrier may lack the decoders' arrivals; then the limit ends the wait).
+      // roles gave up, the copies issued so far still land before the block ends.
       for (int i = 0; ok && i < stages; ++i) {
         ok = mbar_wait_warp(&eb[s], phase ^ 1, abort_flag);
         if (++s == stages) {
@@ -440,7 +479,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     for (int t = first_tile; ok && t < num_tiles; t += step) {
       for (int c = c0; c < c1; ++c, ++n) {
         if ((n & 1) != mine) continue;
-        const int ws = n % C::WSTAGES, as = n % STAGES;
+        const int ws = n % C::WSTAGES, as = n % C::ASTAGES;
         if (!(ok = mbar_wait_warp(&w_full[ws], (n / C::WSTAGES) & 1, abort_flag))) break;
         const uint8_t* stage = smem + C::W0 + ws * C::WSTAGE;
         const uint4* codes = reinterpret_cast<const uint4*>(stage) + rt * LPR;
@@ -454,7 +493,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         for (int i = 0; i < GPC; ++i) coff[i] = sc[i * ROWS].y;
         __syncwarp();
         if (lane == 0) mbar_arrive(&w_empty[ws]);
-        if (!(ok = mbar_wait_warp(&empty[as], ((n / STAGES) & 1) ^ 1, abort_flag))) break;
+        if (!(ok = mbar_wait_warp(&a_empty[as], ((n / C::ASTAGES) & 1) ^ 1, abort_flag))) break;
         fence_after();
         const uint32_t dst = tmem + lanes + C::A0 + as * A_COLS;
 #pragma unroll
@@ -480,7 +519,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[as]);
+        if (lane == 0) mbar_arrive(&a_full[as]);
       }
     }
   } else {
@@ -513,8 +552,9 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         pp += ROWS;
         // wide tiles: this group's half of every granule; else every granule's
         // half of the columns
-        const uint32_t buf = PARTS == 2 ? part : u & 1;
-        ok = mbar_wait_warp(&t_full[buf], PARTS == 2 ? u & 1 : (u >> 1) & 1, abort_flag);
+        const uint32_t st = PARTS == 2 ? 2 * u + part : u;  // number of the step
+        const uint32_t buf = st % C::ACCS;
+        ok = mbar_wait_warp(&t_full[buf], (st / C::ACCS) & 1, abort_flag);
         ++u;
         if (!ok) break;
         fence_after();
@@ -551,7 +591,9 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
           }
         }
       } else {
-        // every MMA and load of this CTA is done: its shared memory is free
+        // once every MMA of this CTA is over (the other group's half as well), the
+        // stages of x have no reader left and take the sums
+        if (!(ok = mbar_wait_warp(&done, 0, abort_flag))) break;
         float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
         for (int i = 0; i < C::PER; ++i) sums[(col0 + i) * BM + rt] = acc[i];
