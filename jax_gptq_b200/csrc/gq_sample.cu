@@ -18,16 +18,26 @@
 // and a term's rounding (2^-46 of the largest) is far below what a float32
 // uniform resolves.  Terms below 2^-(S+1) are zero: they can not be drawn.
 //
-// Split.  A cluster of blocks takes a row, each a contiguous part, each warp a
-// contiguous part of that.  Passes over the row (it stays in L1 and L2):
+// Split.  A cluster of up to 8 blocks takes a row, each a contiguous part, each
+// warp a contiguous part of that.  Passes over the row (from L1 and L2 after the
+// first):
 //   1. the maximum;
-//   2. each warp's sum of e, and with top-k or top-p a histogram (count and
-//      sum) over 512 bins of log2 e;
-//   3. only with a border: the bin it falls in is resolved exactly by radix
-//      passes over the ordered bits of its members;
-//   4. only with filters: each warp's sum of the kept e and its number of
-//      tokens equal to the border;
-//   5. the warp whose part holds u W finds the token.
+//   2. with top-k or top-p the number of tokens in 512 bins of log2 e (found in
+//      float32: any function that keeps the order will do); without top-k each
+//      warp's sum of e;
+//   3. the bins tell down to which one a border can lie: the k-th token's, or the
+//      first by which the sum is at least p (a bin's sum is at least its count
+//      times its smallest e).  Tokens down to there, where they are at most 2048,
+//      are collected and sorted by every block, and the borders read off their
+//      running sum.  Otherwise (flat distributions) top-k's border bin alone is
+//      sorted, then the sums of every bin are taken for top-p and its border bin
+//      is sorted; a bin of more than 2048 (runs of equal logits) is resolved by
+//      radix passes over the ordered bits;
+//   4. with filters each warp's sum of the kept e and its number of tokens equal
+//      to the border;
+//   5. the block that holds u W finds the token in the part of one warp.
+// Reading other blocks' shared memory is slow (a 16 KB histogram of all 8 blocks
+// took 24000 cycles), so little is exchanged, by as many lanes at once as can be.
 #include "gq_common.cuh"
 
 #include <cooperative_groups.h>
@@ -43,9 +53,9 @@ namespace samp {
 
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
-constexpr int BINS = 512;
+constexpr int BINS = 512;   // of log2 e, 11 to a power of two; one a thread
 constexpr int MAX_CL = 8;
-constexpr int LIST = 1024;  // members of a border's bin kept per block
+constexpr int LIST = 2048;  // tokens that are collected and sorted
 
 struct RowParam {  // a setting: one value, or one per row
   const void* rows;
@@ -91,27 +101,33 @@ __device__ __forceinline__ float from_ordered(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
 
-// 2^-y for 0 <= y < 1000, within 2^-48: y is split at the nearest whole number
-// and 2^f, |f| <= 1/2, is the Taylor series of exp(f ln 2) to the 11th power
-// (remainder below 7e-15).
-__device__ __forceinline__ double exp2_neg(double y) {
-  const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the whole part
-  const double s = magic - y;
-  const int n = __double2loint(s);
-  const double x = ((magic - s) - y) * 0.69314718055994530942;
-  double p = 2.505210838544172e-08;                // 1 / 11!
-  p = fma(p, x, 2.755731922398589e-07);
-  p = fma(p, x, 2.755731922398589e-06);
-  p = fma(p, x, 2.48015873015873e-05);
-  p = fma(p, x, 1.984126984126984e-04);
-  p = fma(p, x, 1.388888888888889e-03);
-  p = fma(p, x, 8.333333333333333e-03);
-  p = fma(p, x, 4.1666666666666664e-02);
-  p = fma(p, x, 1.6666666666666666e-01);
-  p = fma(p, x, 0.5);
-  p = fma(p, x, 1.0);
-  p = fma(p, x, 1.0);
-  return __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+// 2^-y for 0 <= y < 1000, within 2^-47 of it: y is split at the nearest whole
+// number and 2^f, |f| <= 1/2, is the Taylor series of exp(f ln 2) to the 11th power
+// (remainder below 7e-15).  N at a time, step by step: one alone is a chain of 18
+// dependent float64 operations, and four warps a scheduler do not hide that.
+template <int N>
+__device__ __forceinline__ void exp2_neg(const double (&y)[N], double (&out)[N]) {
+  constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the whole part
+  constexpr double c[12] = {1.0, 1.0, 0.5, 1.6666666666666666e-01, 4.1666666666666664e-02,
+                            8.333333333333333e-03, 1.388888888888889e-03, 1.984126984126984e-04,
+                            2.48015873015873e-05, 2.755731922398589e-06, 2.755731922398589e-07,
+                            2.505210838544172e-08};  // 1 / n!
+  double x[N];
+  int n[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const double s = magic - y[i];
+    n[i] = __double2loint(s);
+    x[i] = ((magic - s) - y[i]) * 0.69314718055994530942;
+    out[i] = c[11];
+  }
+#pragma unroll
+  for (int k = 10; k >= 0; --k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = fma(out[i], x[i], c[k]);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    out[i] = __hiloint2double(__double2hiint(out[i]) + (n[i] << 20), __double2loint(out[i]));
 }
 
 struct Row {
@@ -119,17 +135,31 @@ struct Row {
   double limit;  // terms with log2 e below -limit are zero
   double scale;
   // distance below the maximum in powers of two; false where the term is zero
+  // (y is then any number)
   __device__ __forceinline__ bool distance(float l, double& y) const {
     const double v = (double)l;
     y = v == mx ? 0.0 : (mx - v) * c;
     return y < limit;  // false for NaN
   }
-  __device__ __forceinline__ uint64_t fixed(double y) const {
-    const double t = fma(exp2_neg(y), scale, 4503599627370496.0);  // + 2^52: whole number in the low bits
-    return (uint64_t)__double_as_longlong(t) & 0xfffffffffffffull;
+  // the terms as whole numbers, 0 where !have
+  template <int N>
+  __device__ __forceinline__ void fixed(const double (&y)[N], const bool (&have)[N],
+                                        uint64_t (&f)[N]) const {
+    double e[N];
+    exp2_neg(y, e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const double t = fma(e[i], scale, 4503599627370496.0);  // + 2^52: whole number in the low bits
+      f[i] = have[i] ? (uint64_t)__double_as_longlong(t) & 0xfffffffffffffull : 0;
+    }
   }
-  __device__ __forceinline__ int bin(double y) const {
-    return min(BINS - 1, (int)((float)y * 11.f));  // 46.5 powers of two
+  __device__ __forceinline__ uint64_t fixed(float l) const {
+    double y[1];
+    const bool have[1] = {distance(l, y[0])};
+    uint64_t f[1];
+    if (!have[0]) y[0] = 0.0;
+    fixed(y, have, f);
+    return f[0];
   }
 };
 
@@ -174,35 +204,39 @@ struct Border {
 };
 
 struct Shared {
-  unsigned long long mass[BINS];       // histogram over log2 e
-  uint32_t count[BINS];
-  unsigned long long rmass[2][256];    // a radix pass, two buffers in turn
-  uint32_t rcount[2][256];
+  unsigned long long mass[BINS];       // histogram over log2 e: sums
+  uint32_t count[BINS];                // and tokens
+  union {
+    uint32_t keys[LIST];               // collected from the whole row, sorted
+    struct {
+      unsigned long long rmass[2][256];  // a radix pass, two buffers in turn
+      uint32_t rcount[2][256];
+    } radix;
+  };
+  uint32_t list[LIST];                 // collected in this block
+  uint32_t list_n, kmin, kmax;
   uint64_t wmass[WARPS];               // per warp: what the draw walks through
   uint32_t wties[WARPS];
-  uint32_t list[LIST];
-  uint32_t list_n, kmin, kmax;
   float mx[WARPS];
   uint32_t amax[WARPS];
-  // scratch of the scans over bins and digits
-  unsigned long long smass[WARPS];
+  unsigned long long smass[WARPS];     // scratch of the scans
   uint32_t scount[WARPS];
   float block_max;
   uint32_t block_arg;
   unsigned long long all_mass[MAX_CL * WARPS];  // every warp of the cluster
   uint32_t all_ties[MAX_CL * WARPS];
   int pick_warp;
-  uint32_t pick_ties;
+  uint32_t pick_ties, pick_all_ties;
   unsigned long long pick_before, pick_total;
   int found;
-  uint32_t found_count;
-  unsigned long long found_mass;
-  uint32_t found_own;
-  unsigned long long found_own_mass;
+  uint32_t found_count, found_own;
+  unsigned long long found_mass, found_own_mass;
+  int hit, last;
+  double hit_y, last_y;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   constexpr int VEC = Units<T>::VEC;
   __shared__ Shared sh;
   cg::cluster_group cl = cg::this_cluster();
@@ -213,8 +247,29 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
   const Units<T> un(row, a.vocab);
   // this warp's units
   const int b0 = (int)((int64_t)un.count * rank / CL), b1 = (int)((int64_t)un.count * (rank + 1) / CL);
-  const int w0 = b0 + (int)((int64_t)(b1 - b0) * warp / WARPS);
-  const int w1 = b0 + (int)((int64_t)(b1 - b0) * (warp + 1) / WARPS);
+  auto warp_begin = [&](int w) { return b0 + (int)((int64_t)(b1 - b0) * w / WARPS); };
+  const int w0 = warp_begin(warp), w1 = warp_begin(warp + 1);
+  // f(values, index of the first) for this lane's tokens, a unit at a time, NaN
+  // where there is none; the next unit is read ahead
+  auto each_unit = [&](auto&& f) {
+    float x[VEC], next[VEC];
+    int q = w0 + lane;
+    if (q < w1) un.load(q, x);
+    for (; q < w1; q += 32) {
+      if (q + 32 < w1) un.load(q + 32, next);
+      f(x, q * VEC - un.shift);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[e] = next[e];
+    }
+  };
+  auto each_token = [&](auto&& f) {
+    each_unit([&](const float (&x)[VEC], int i) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f(x[e], i + e);
+    });
+  };
+  // the same field of block c, read by lane c of every warp
+  auto peer = [&](int c) { return cl.map_shared_rank(&sh, c); };
 
   const double temp = row_value(a.temperature, r);
   const double kd = row_value(a.top_k, r);
@@ -225,16 +280,12 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
   // ---- 1. the maximum (and for temperature 0 its first index)
   float mx = -INFINITY;
   uint32_t arg = 0xffffffffu;
-  for (int q = w0 + lane; q < w1; q += 32) {
-    float x[VEC];
-    un.load(q, x);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (x[e] > mx) {  // indices grow along a lane's walk: the first one stays
-        mx = x[e];
-        arg = (uint32_t)(q * VEC - un.shift + e);
-      }
-  }
+  each_token([&](float x, int i) {
+    if (x > mx) {  // indices grow along a lane's walk: the first one stays
+      mx = x;
+      arg = (uint32_t)i;
+    }
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float om = __shfl_xor_sync(0xffffffffu, mx, o);
@@ -248,41 +299,46 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
     sh.mx[warp] = mx;
     sh.amax[warp] = arg;
   }
-  for (int i = tid; i < BINS; i += THREADS) {
-    sh.mass[i] = 0;
-    sh.count[i] = 0;
-  }
-  if (tid < 256) {
-    sh.rmass[0][tid] = 0;
-    sh.rcount[0][tid] = 0;
-  }
+  sh.mass[tid] = 0;
+  sh.count[tid] = 0;
   if (tid == 0) {
     sh.list_n = 0;
     sh.kmin = 0xffffffffu;
     sh.kmax = 0;
+    sh.hit = sh.last = -1;
   }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < WARPS; ++w)
-      if (sh.mx[w] > mx || (sh.mx[w] == mx && sh.amax[w] < arg)) {
-        mx = sh.mx[w];
-        arg = sh.amax[w];
+  if (warp == 0) {
+    mx = lane < WARPS ? sh.mx[lane] : -INFINITY;
+    arg = lane < WARPS ? sh.amax[lane] : 0xffffffffu;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, mx, o);
+      const uint32_t oa = __shfl_xor_sync(0xffffffffu, arg, o);
+      if (om > mx || (om == mx && oa < arg)) {
+        mx = om;
+        arg = oa;
       }
-    sh.block_max = mx;
-    sh.block_arg = arg;
+    }
+    if (lane == 0) {
+      sh.block_max = mx;
+      sh.block_arg = arg;
+    }
   }
   cl.sync();
-  mx = -INFINITY;
-  arg = 0xffffffffu;
-  for (int c = 0; c < CL; ++c) {
-    const Shared* o = cl.map_shared_rank(&sh, c);
-    const float om = o->block_max;
-    const uint32_t oa = o->block_arg;
+  mx = lane < CL ? peer(lane)->block_max : -INFINITY;
+  arg = lane < CL ? peer(lane)->block_arg : 0xffffffffu;
+#pragma unroll
+  for (int o = MAX_CL / 2; o > 0; o >>= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, mx, o);
+    const uint32_t oa = __shfl_xor_sync(0xffffffffu, arg, o);
     if (om > mx || (om == mx && oa < arg)) {
       mx = om;
       arg = oa;
     }
   }
+  mx = __shfl_sync(0xffffffffu, mx, 0);
+  arg = __shfl_sync(0xffffffffu, arg, 0);
   const bool none = !(mx > -INFINITY);
   if (none || !(temp > 0.0)) {
     if (rank == 0 && tid == 0) {
@@ -297,296 +353,424 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
   rw.c = fmin(1.4426950408889634 / temp, 1e300);
   rw.scale = a.scale;
   rw.limit = (double)(((__double2hiint(a.scale) >> 20) & 0x7ff) - 1023) + 1.0;  // S + 1
+  const float cf = (float)fmin(rw.c, 3e38);
+  // bin of a token; the last bin holds only terms that are zero (46.45 powers of
+  // two below the largest and further), and whatever is no token at all
+  auto bin_of = [&](float l) {
+    const float y = l == mx ? 0.f : (mx - l) * cf;
+    return min(BINS - 1, (int)(fminf(y, 50.f) * 11.f));
+  };
   const bool by_k = kd >= 1.0 && kd < (double)a.vocab;
   const uint32_t k = by_k ? (uint32_t)kd : 0;
   const bool by_p = p < 1.0;
   const bool by_min = mp > 0.0;
-  const double floor_e = fmin(mp, 1.0);  // the largest term stays whatever min_p is
+  // e >= min_p in powers of two below the largest; the largest itself stays
+  const double floor_y = by_min ? fmax(-log2(mp), 0.0) : 0.0;
 
-  // ---- 2. sums and histogram
-  {
+  // ---- 2. sums, tokens per bin
+  if (by_k || by_p)
+    each_token([&](float x, int) {
+      const int b = bin_of(x);
+      if (b < BINS - 1) atomicAdd(&sh.count[b], 1u);
+    });
+  auto sum_terms = [&] {  // each warp's sum of e
     uint64_t sum = 0;
-    const bool hist = by_k || by_p;
-    for (int q = w0 + lane; q < w1; q += 32) {
-      float x[VEC];
-      un.load(q, x);
+    each_unit([&](const float (&x)[VEC], int) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        double y;
-        if (!rw.distance(x[e], y)) continue;
-        const uint64_t f = rw.fixed(y);
-        sum += f;
-        if (hist) {
-          const int b = rw.bin(y);
-          atomicAdd(&sh.mass[b], (unsigned long long)f);
-          atomicAdd(&sh.count[b], 1u);
+      for (int h = 0; h < VEC; h += 4) {
+        double y[4];
+        bool have[4];
+        uint64_t f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          have[e] = rw.distance(x[h + e], y[e]);
+          y[e] = have[e] ? y[e] : 0.0;
         }
+        rw.fixed(y, have, f);
+        sum += f[0] + f[1] + f[2] + f[3];
       }
-    }
+    });
     sum = warp_sum64(sum);
-    if (lane == 0) {
-      sh.wmass[warp] = sum;
-      sh.wties[warp] = 0;
-    }
-  }
+    if (lane == 0) sh.wmass[warp] = sum;
+  };
+  if (!by_k) sum_terms();
+  if (lane == 0) sh.wties[warp] = 0;
   cl.sync();
 
   // ---- 3. borders
   Border border{0, 0xffffffffu};  // everything
-  if (by_k || by_p) {
-    unsigned long long hm = 0;  // this thread's bin over the whole row
-    uint32_t hc = 0;
-    for (int c = 0; c < CL; ++c) {
-      const Shared* o = cl.map_shared_rank(&sh, c);
-      hm += o->mass[tid];
-      hc += o->count[tid];
-    }
-    // exclusive prefixes over bins (the largest e first)
-    auto scan = [&](unsigned long long m, uint32_t n, int width, unsigned long long& pm, uint32_t& pn) {
-      unsigned long long im = m;
-      uint32_t in = n;
+  // exclusive prefixes over the threads, and the totals
+  auto scan = [&](unsigned long long m, uint32_t n, unsigned long long& pm, uint32_t& pn,
+                  unsigned long long& tm, uint32_t& tn) {
+    unsigned long long im = m;
+    uint32_t in = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long tm = __shfl_up_sync(0xffffffffu, im, o);
-        const uint32_t tn = __shfl_up_sync(0xffffffffu, in, o);
-        if (lane >= o) {
-          im += tm;
-          in += tn;
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long vm = __shfl_up_sync(0xffffffffu, im, o);
+      const uint32_t vn = __shfl_up_sync(0xffffffffu, in, o);
+      if (lane >= o) {
+        im += vm;
+        in += vn;
+      }
+    }
+    __syncthreads();
+    if (lane == 31) {
+      sh.smass[warp] = im;
+      sh.scount[warp] = in;
+    }
+    __syncthreads();
+    unsigned long long wm = lane < WARPS ? sh.smass[lane] : 0;
+    uint32_t wn = lane < WARPS ? sh.scount[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < WARPS; o <<= 1) {
+      const unsigned long long vm = __shfl_up_sync(0xffffffffu, wm, o);
+      const uint32_t vn = __shfl_up_sync(0xffffffffu, wn, o);
+      if (lane >= o) {
+        wm += vm;
+        wn += vn;
+      }
+    }
+    tm = __shfl_sync(0xffffffffu, wm, WARPS - 1);
+    tn = __shfl_sync(0xffffffffu, wn, WARPS - 1);
+    const unsigned long long bm = __shfl_sync(0xffffffffu, wm, max(warp - 1, 0));
+    const uint32_t bn = __shfl_sync(0xffffffffu, wn, max(warp - 1, 0));
+    pm = im - m + (warp > 0 ? bm : 0);
+    pn = in - n + (warp > 0 ? bn : 0);
+  };
+  // what the one thread that found something (what >= 0) says to all
+  auto tell = [&](int what, uint32_t n, unsigned long long m, uint32_t own, unsigned long long own_m) {
+    __syncthreads();
+    if (tid == 0) sh.found = -1;
+    __syncthreads();
+    if (what >= 0) {
+      sh.found = what;
+      sh.found_count = n;
+      sh.found_mass = m;
+      sh.found_own = own;
+      sh.found_own_mass = own_m;
+    }
+    __syncthreads();
+    return sh.found;
+  };
+  // of `own` equal tokens, before which `msum` lies, those that begin before the target
+  auto staying = [&](uint32_t own, unsigned long long each, unsigned long long msum, double target) {
+    if (each == 0) return own;
+    const double room = (target - (double)msum) / (double)each;
+    uint32_t j = room >= (double)own ? own : room > 0.0 ? (uint32_t)room : 0u;
+    while (j > 0 && !((double)(msum + (unsigned long long)(j - 1) * each) < target)) --j;
+    while (j < own && (double)(msum + (unsigned long long)j * each) < target) ++j;
+    return j;
+  };
+  // Collects the keys of this row's tokens that `pred` picks; the number of them
+  // over the whole row, of which the first LIST are in this block's `list`s.
+  auto collect = [&](auto&& pred) {
+    __syncthreads();
+    if (tid == 0) {
+      sh.list_n = 0;
+      sh.kmin = 0xffffffffu;
+      sh.kmax = 0;
+    }
+    __syncthreads();
+    each_token([&](float x, int) {
+      if (!pred(x)) return;
+      const uint32_t key = ordered(x);
+      const uint32_t at = atomicAdd(&sh.list_n, 1u);
+      if (at < LIST) sh.list[at] = key;
+      atomicMin(&sh.kmin, key);
+      atomicMax(&sh.kmax, key);
+    });
+    cl.sync();
+    const uint32_t n = __reduce_add_sync(0xffffffffu, lane < CL ? peer(lane)->list_n : 0);
+    if (n > LIST) cl.sync();  // the lists are not read further and may be begun anew
+    return n;
+  };
+  // The collected keys (n <= LIST) of all blocks in `keys`, largest first.
+  auto sorted = [&](uint32_t n) {
+    const uint32_t mine = lane < CL ? peer(lane)->list_n : 0;
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < MAX_CL; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    uint32_t size = 64;
+    while (size < n) size *= 2;
+    for (uint32_t i = tid; i < ((size + 31) & ~31u); i += THREADS) {
+      uint32_t key = 0;  // below every key
+      uint32_t c = 0, from = 0;
+#pragma unroll
+      for (int o = 0; o < MAX_CL; ++o) {
+        const uint32_t end = __shfl_sync(0xffffffffu, upto, o);
+        if (o < CL && i >= end) {
+          c = o + 1;
+          from = end;
         }
       }
-      __syncthreads();
-      if (lane == 31) {
-        sh.smass[warp] = im;
-        sh.scount[warp] = in;
-      }
-      __syncthreads();
-      pm = im - m;
-      pn = in - n;
-      for (int w = 0; w < warp; ++w) {
-        pm += sh.smass[w];
-        pn += sh.scount[w];
-      }
-    };
-    unsigned long long bm, total_m = 0;
-    uint32_t bc, total_c = 0;
-    scan(hm, hc, BINS, bm, bc);
-    for (int w = 0; w < WARPS; ++w) {
-      total_m += sh.smass[w];
-      total_c += sh.scount[w];
+      if (i < n) key = peer(c)->list[i - from];
+      if (i < size) sh.keys[i] = key;
     }
-    int buf = 0;
-    // The key at which the border lies inside bin `fb`, before which `cnt`
-    // tokens of mass `msum` lie.  by_mass: the first token whose preceding mass
-    // reaches `target` is the first one out; else `k` tokens stay.
-    auto resolve = [&](bool by_mass, int fb, uint32_t cnt, unsigned long long msum, double target,
-                       Border& out, unsigned long long& kept_mass) {
-      if (tid == 0) {
-        sh.list_n = 0;
-        sh.kmin = 0xffffffffu;
-        sh.kmax = 0;
-      }
-      __syncthreads();
-      uint32_t lo = 0xffffffffu, hi = 0;
-      for (int q = w0 + lane; q < w1; q += 32) {
-        float x[VEC];
-        un.load(q, x);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          double y;
-          if (!rw.distance(x[e], y) || rw.bin(y) != fb) continue;
-          const uint32_t key = ordered(x[e]);
-          lo = min(lo, key);
-          hi = max(hi, key);
-          const uint32_t at = atomicAdd(&sh.list_n, 1u);
-          if (at < LIST) sh.list[at] = key;
+    // bitonic network; pairs up to 32 apart stay inside a warp's 64 keys
+    uint32_t last = 64;
+    for (uint32_t k2 = 2; k2 <= size; k2 *= 2)
+      for (uint32_t j = k2 / 2; j > 0; j /= 2) {
+        if (j > 32 || last > 32) __syncthreads();
+        else __syncwarp();
+        last = j;
+        for (uint32_t t = tid; t < size / 2; t += THREADS) {
+          const uint32_t i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
+          const uint32_t x = sh.keys[i], y = sh.keys[i + j];
+          if (((i & k2) == 0) == (x < y)) {
+            sh.keys[i] = y;
+            sh.keys[i + j] = x;
+          }
         }
       }
-      lo = __reduce_min_sync(0xffffffffu, lo);
-      hi = __reduce_max_sync(0xffffffffu, hi);
-      if (lane == 0) {
-        atomicMin(&sh.kmin, lo);
-        atomicMax(&sh.kmax, hi);
-      }
+    __syncthreads();
+  };
+  // The terms of the first n sorted keys, EACH a thread, with their running sum; and
+  // the number of the last one that begins before `target` (at least the first).
+  constexpr int EACH = LIST / THREADS;
+  auto running = [&](uint32_t n, unsigned long long (&f)[EACH], unsigned long long& pm,
+                     unsigned long long& total) {
+#pragma unroll
+    for (int h = 0; h < EACH; ++h) {
+      const uint32_t i = EACH * tid + h;
+      f[h] = i < n ? rw.fixed(from_ordered(sh.keys[i])) : 0;
+    }
+    uint32_t pn, tn;
+    scan(f[0] + f[1] + f[2] + f[3], 0, pm, pn, total, tn);
+  };
+  auto last_before = [&](uint32_t n, const unsigned long long (&f)[EACH], unsigned long long pm,
+                         double target) {
+    uint32_t stays = 0;
+#pragma unroll
+    for (int h = 0; h < EACH; ++h) {
+      if (EACH * tid + h < n && (double)pm < target) ++stays;
+      pm += f[h];
+    }
+    unsigned long long qm, tm;
+    uint32_t pn, tn;
+    scan(0, stays, qm, pn, tm, tn);
+    return max(tn, 1u) - 1;
+  };
+  auto border_at = [&](uint32_t place, Border& out) {  // after sorted key number `place`
+    out.key = sh.keys[place];
+    uint32_t ties = 0;
+    for (uint32_t i = tid; i <= place; i += THREADS) ties += sh.keys[i] == out.key;
+    unsigned long long pm, tm;
+    uint32_t pn;
+    scan(0, ties, pm, pn, tm, out.ties);
+  };
+  static_assert(EACH == 4, "sums of four");
+  // Radix passes over the members of bin `fb` with keys above `above`, before which
+  // `cnt` tokens of mass `msum` lie, with digits of 8 bits from the highest bit in
+  // which they differ.  by_mass: the tokens that begin before `target` stay; else
+  // `k` tokens do.
+  auto radix = [&](bool by_mass, int fb, uint32_t above, uint32_t cnt, unsigned long long msum,
+                   double target, Border& out) {
+    uint32_t lo = lane < CL ? peer(lane)->kmin : 0xffffffffu, hi = lane < CL ? peer(lane)->kmax : 0u;
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    int bits = 32 - __clz(lo ^ hi), buf = 0;
+    uint32_t prefix = bits >= 32 ? 0 : (hi >> bits) << bits;
+    uint32_t own = 0;               // tokens equal to the key so far
+    unsigned long long own_mass = 0;
+    if (tid < 256) {
+      sh.radix.rmass[0][tid] = 0;
+      sh.radix.rcount[0][tid] = 0;
+    }
+    __syncthreads();
+    bool first = true;
+    while (bits > 0 || first) {
+      first = false;
+      const int shift = max(0, bits - 8);
+      const uint32_t dmask = bits > 0 ? ((bits >= 32 ? 0xffffffffu : (1u << bits) - 1u) >> shift) : 0u;
+      const uint32_t high = bits >= 32 ? 0u : ~((1u << bits) - 1u);
+      each_token([&](float x, int) {
+        if (bin_of(x) != fb) return;
+        const uint32_t key = ordered(x);
+        if (key <= above || (key & high) != (prefix & high)) return;
+        const uint32_t d = dmask - ((key >> shift) & dmask);  // largest first
+        atomicAdd(&sh.radix.rcount[buf][d], 1u);
+        if (by_mass) atomicAdd(&sh.radix.rmass[buf][d], (unsigned long long)rw.fixed(x));
+      });
       cl.sync();
-      for (int c = 0; c < CL; ++c) {
-        const Shared* o = cl.map_shared_rank(&sh, c);
-        lo = min(lo, o->kmin);
-        hi = max(hi, o->kmax);
+      unsigned long long m = 0;
+      uint32_t n = 0;
+      if (tid < 256) {
+        for (int c = 0; c < CL; ++c) {
+          m += peer(c)->radix.rmass[buf][tid];
+          n += peer(c)->radix.rcount[buf][tid];
+        }
+        sh.radix.rmass[buf ^ 1][tid] = 0;  // its last readers passed the sync above
+        sh.radix.rcount[buf ^ 1][tid] = 0;
       }
-      const bool listed = sh.list_n <= LIST;
-      const int members = listed ? (int)sh.list_n : 0;
-      // digits of 8 bits from the highest bit in which the members differ
-      int bits = 32 - __clz(lo ^ hi);
-      uint32_t prefix = bits >= 32 ? 0 : (hi >> bits) << bits;
-      uint32_t own = 0;               // tokens equal to the key so far
-      unsigned long long own_mass = 0;
-      bool first = true;
-      while (bits > 0 || first) {
-        first = false;
-        const int shift = max(0, bits - 8);
-        const uint32_t dmask = bits > 0 ? ((bits >= 32 ? 0xffffffffu : (1u << bits) - 1u) >> shift) : 0u;
-        const uint32_t high = bits >= 32 ? 0u : ~((1u << bits) - 1u);
-        auto put = [&](uint32_t key, uint64_t f) {
-          const uint32_t d = dmask - ((key >> shift) & dmask);  // largest first
-          atomicAdd(&sh.rcount[buf][d], 1u);
-          atomicAdd(&sh.rmass[buf][d], (unsigned long long)f);
-        };
-        if (listed) {
-          for (int i = tid; i < members; i += THREADS) {
-            const uint32_t key = sh.list[i];
-            if ((key & high) != (prefix & high)) continue;
-            double y;
-            rw.distance(from_ordered(key), y);
-            put(key, rw.fixed(y));
-          }
-        } else {
-          for (int q = w0 + lane; q < w1; q += 32) {
-            float x[VEC];
-            un.load(q, x);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              double y;
-              if (!rw.distance(x[e], y) || rw.bin(y) != fb) continue;
-              const uint32_t key = ordered(x[e]);
-              if ((key & high) == (prefix & high)) put(key, rw.fixed(y));
-            }
-          }
-        }
-        cl.sync();
-        unsigned long long m = 0;
-        uint32_t n = 0;
-        if (tid < 256) {
-          for (int c = 0; c < CL; ++c) {
-            const Shared* o = cl.map_shared_rank(&sh, c);
-            m += o->rmass[buf][tid];
-            n += o->rcount[buf][tid];
-          }
-          sh.rmass[buf ^ 1][tid] = 0;  // the last readers of that buffer passed the sync above
-          sh.rcount[buf ^ 1][tid] = 0;
-        }
-        unsigned long long pm;
-        uint32_t pn;
-        scan(m, n, 256, pm, pn);
-        pm += msum;
-        pn += cnt;
-        // the digit that holds the border: for k the one with the k-th token,
-        // for p the last one that begins before the target
-        const bool mine = n > 0 && (by_mass ? (double)pm < target && !((double)(pm + m) < target)
-                                            : pn < k && pn + n >= k);
-        if (tid == 0) sh.found = -1;
-        __syncthreads();
-        if (mine) {
-          sh.found = tid;
-          sh.found_count = pn;
-          sh.found_mass = pm;
-          sh.found_own = n;
-          sh.found_own_mass = m;
-        }
-        __syncthreads();
-        const int d = max(sh.found, 0);
-        cnt = sh.found_count;
-        msum = sh.found_mass;
-        own = sh.found_own;
-        own_mass = sh.found_own_mass;
-        prefix = (prefix & high) | ((dmask - (uint32_t)d) << shift);
-        buf ^= 1;
-        bits = shift;
-        __syncthreads();
-      }
-      // `own` tokens share the key; their terms are equal
-      const unsigned long long each = own ? own_mass / own : 0;
-      uint32_t stay;
-      if (by_mass) {
-        // token number j of them stays while msum + j * each < target
-        stay = own;
-        if (each > 0) {
-          const double room = (target - (double)msum) / (double)each;
-          uint32_t j = room >= (double)own ? own : (uint32_t)room;
-          while (j > 0 && !((double)(msum + (unsigned long long)(j - 1) * each) < target)) --j;
-          while (j < own && (double)(msum + (unsigned long long)j * each) < target) ++j;
-          stay = j;
-        }
-      } else {
-        stay = min(own, k - cnt);
-      }
-      out.key = prefix;
-      out.ties = stay;
-      kept_mass = msum + (unsigned long long)stay * each;
-    };
+      unsigned long long pm, tm;
+      uint32_t pn, tn;
+      scan(m, n, pm, pn, tm, tn);
+      pm += msum;
+      pn += cnt;
+      // the digit that holds the k-th token, or the last one that begins before the target
+      const bool mine = n > 0 && (by_mass ? (double)pm < target && !((double)(pm + m) < target)
+                                          : pn < k && pn + n >= k);
+      const int d = max(tell(mine ? tid : -1, pn, pm, n, m), 0);
+      cnt = sh.found_count;
+      msum = sh.found_mass;
+      own = sh.found_own;
+      own_mass = sh.found_own_mass;
+      prefix = (prefix & high) | ((dmask - (uint32_t)d) << shift);
+      buf ^= 1;
+      bits = shift;
+    }
+    cl.sync();  // the buffers are read: a later call may use their place
+    out.key = prefix;
+    out.ties = by_mass ? staying(own, own ? own_mass / own : 0, msum, target) : min(own, k - cnt);
+  };
 
-    unsigned long long zk = total_m;  // mass that top-k leaves
-    bool cut_k = by_k && total_c > k;
+  if (by_k || by_p) {
+    // this thread's bin over the whole row: tokens, and the least that its sum can be
+    // (count * 2^-((bin + 1) / 11), with room for roundings)
+    uint32_t hc = 0, bc, total_c;
+    unsigned long long bm, tm;
+#pragma unroll
+    for (int c = 0; c < MAX_CL; ++c)
+      if (c < CL) hc += peer(c)->count[tid];
+    const unsigned long long least = (unsigned long long)(
+        hc * (double)exp2f(-((float)tid + 1.01f) / 11.f) * 0.9999 * rw.scale);
+    scan(least, hc, bm, bc, tm, total_c);
+    const bool cut_k = by_k && total_c > k;
+    if (by_k && !cut_k && by_p) {  // fewer tokens than k: top-p over all of them
+      sum_terms();
+      cl.sync();
+    }
+    unsigned long long z = 0;  // mass that top-k leaves
+    double target = 0.0;
+    if (by_p && !cut_k) {
+      for (int i = lane; i < CL * WARPS; i += 32) z += peer(i / WARPS)->wmass[i % WARPS];
+      z = warp_sum64(z);
+      target = fmax(p, 0.0) * (double)z;
+    }
+    int limit = -1;          // the bin down to which a border can lie
+    uint32_t through = 0;    // tokens down to there
     if (cut_k) {
-      const bool mine = bc < k && bc + hc >= k;
-      if (mine) {
-        sh.found = tid;
-        sh.found_count = bc;
-        sh.found_mass = bm;
-      }
-      __syncthreads();
-      const int fb = sh.found;
-      const uint32_t cnt = sh.found_count;
-      const unsigned long long msum = sh.found_mass;
-      __syncthreads();
-      resolve(false, fb, cnt, msum, 0.0, border, zk);
-    }
-    if (by_p) {
-      const double target = fmax(p, 0.0) * (double)zk;
-      // the last bin that begins before the target; the first token stays even at p = 0
-      const bool mine = hc > 0 && (double)bm < target && !((double)(bm + hm) < target);
-      if (tid == 0) sh.found = -1;
-      __syncthreads();
-      if (mine) {
-        sh.found = tid;
-        sh.found_count = bc;
-        sh.found_mass = bm;
-      }
-      __syncthreads();
-      const int fb = sh.found;
-      const uint32_t cnt = sh.found_count;
-      const unsigned long long msum = sh.found_mass;
-      __syncthreads();
-      Border bp{ordered(mx), 1};
-      if (fb >= 0) {
-        unsigned long long ignored;
-        resolve(true, fb, cnt, msum, target, bp, ignored);
-        if (bp.key > border.key || (bp.key == border.key && bp.ties < border.ties)) border = bp;
-      } else if (!(target > 0.0)) {
-        border = bp;
+      limit = tell(bc < k && bc + hc >= k ? tid : -1, bc, 0, bc + hc, 0);
+      through = sh.found_own;
+    } else if (by_p) {
+      limit = tell((double)bm < target && !((double)(bm + least) < target) ? tid : -1, 0, 0, bc + hc, 0);
+      through = sh.found_own;
+      if (limit < 0) {
+        limit = BINS - 2;
+        through = total_c;
       }
     }
+    const uint32_t k_before = sh.found_count;  // with cut_k: tokens of the bins before
+    if (limit >= 0) {
+      uint32_t n = LIST + 1;
+      if (through <= LIST) {
+        // the value down to which to collect, a little too far rather than too short
+        const float d = ((float)limit + 1.f) * 1.0001f / (11.f * cf);
+        float thr = mx;
+        if (mx < INFINITY) {
+          thr = mx - d;
+          if (thr > -INFINITY) thr -= fabsf(thr) * 3e-7f;
+        }
+        n = collect([&](float x) { return x >= thr && x > -INFINITY; });
+      }
+      if (n <= LIST) {
+        sorted(n);
+        const uint32_t nk = cut_k ? min(k, n) : n;
+        uint32_t place = nk - 1;
+        if (by_p) {
+          unsigned long long f[EACH], pm, total;
+          running(nk, f, pm, total);
+          if (cut_k) target = fmax(p, 0.0) * (double)total;
+          place = last_before(nk, f, pm, target);
+        }
+        border_at(place, border);
+      } else {
+        if (cut_k) {
+          n = collect([&](float x) { return bin_of(x) == limit; });
+          if (n <= LIST) {
+            sorted(n);
+            border_at(k - k_before - 1, border);
+          } else {
+            radix(false, limit, 0u, k_before, 0, 0.0, border);
+          }
+        }
+        if (by_p) {
+          each_token([&](float x, int) {
+            const int b = bin_of(x);
+            if (b <= limit && (!cut_k || ordered(x) > border.key))
+              atomicAdd(&sh.mass[b], (unsigned long long)rw.fixed(x));
+          });
+          cl.sync();
+          unsigned long long hm = 0, pm;
+          uint32_t pn, tn;
+#pragma unroll
+          for (int c = 0; c < MAX_CL; ++c)
+            if (c < CL) hm += peer(c)->mass[tid];
+          scan(hm, 0, pm, pn, tm, tn);
+          const unsigned long long each = cut_k ? rw.fixed(from_ordered(border.key)) : 0;
+          if (cut_k) target = fmax(p, 0.0) * (double)(tm + border.ties * each);
+          // the last bin that begins before the target
+          const int fb = tell((double)pm < target && !((double)(pm + hm) < target) ? tid : -1, 0, pm, 0, 0);
+          const unsigned long long msum = sh.found_mass;
+          if (fb >= 0) {
+            const uint32_t above = cut_k ? border.key : 0u;
+            n = collect([&](float x) { return bin_of(x) == fb && ordered(x) > above; });
+            if (n <= LIST) {
+              sorted(n);
+              unsigned long long f[EACH], total;
+              running(n, f, pm, total);
+              border_at(last_before(n, f, pm + msum, target), border);
+            } else {
+              radix(true, fb, above, 0, msum, target, border);
+            }
+          } else if (cut_k) {  // among the tokens equal to top-k's border
+            border.ties = staying(border.ties, each, tm, target);
+          }
+        }
+      }
+    }
+    // p = 0, or sums that leave the first token alone
+    if (by_p && !(target > 0.0)) border = Border{ordered(mx), 1};
   }
 
   // ---- 4. what is kept, per warp
-  const bool filtered = border.key != 0 || by_min;
-  auto kept = [&](float l, double& y, uint64_t& f, bool& tie) {
-    tie = false;
-    if (!rw.distance(l, y)) return false;
-    if (border.key != 0) {
-      const uint32_t key = ordered(l);
-      if (key < border.key) return false;
-      tie = key == border.key;
-    }
-    if (by_min && y != 0.0 && exp2_neg(y) < floor_e) return false;
-    f = rw.fixed(y);
-    return true;
+  const bool filtered = border.key != 0 || by_min || by_k;
+  const float border_value = border.key != 0 ? from_ordered(border.key) : -INFINITY;
+  auto kept = [&](float l, double& y, bool& tie) {
+    tie = l == border_value;
+    return l >= border_value && rw.distance(l, y) && !(by_min && y > floor_y);
   };
   if (filtered) {
     uint64_t sum = 0;
     uint32_t ties = 0;
-    for (int q = w0 + lane; q < w1; q += 32) {
-      float x[VEC];
-      un.load(q, x);
+    each_unit([&](const float (&x)[VEC], int) {
+      bool any = false;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        double y;
-        uint64_t f;
-        bool tie;
-        if (!kept(x[e], y, f, tie)) continue;
-        if (tie) ++ties;
-        else sum += f;
+      for (int e = 0; e < VEC; ++e) any |= x[e] >= border_value;
+      if (!any) return;
+#pragma unroll
+      for (int h = 0; h < VEC; h += 4) {
+        double y[4];
+        bool have[4];
+        uint64_t f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bool tie;
+          have[e] = kept(x[h + e], y[e], tie);
+          if (have[e] && tie && border.key != 0) {
+            ++ties;
+            have[e] = false;
+          }
+          y[e] = have[e] ? y[e] : 0.0;
+        }
+        if (!(have[0] || have[1] || have[2] || have[3])) continue;
+        rw.fixed(y, have, f);
+        sum += f[0] + f[1] + f[2] + f[3];
       }
-    }
+    });
     sum = warp_sum64(sum);
     ties = __reduce_add_sync(0xffffffffu, ties);
     if (lane == 0) {
@@ -599,10 +783,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
   // ---- 5. the draw: warp 0 of every block finds which of the cluster's warps,
   // in order, passes u W (or is the last with any mass)
   uint64_t each = 0;  // term of a token equal to the border
-  if (border.key != 0) {
-    double y;
-    if (rw.distance(from_ordered(border.key), y)) each = rw.fixed(y);
-  }
+  if (border.key != 0) each = rw.fixed(from_ordered(border.key));
   if (tid < CL * WARPS) {
     const Shared* o = cl.map_shared_rank(&sh, tid / WARPS);
     sh.all_mass[tid] = o->wmass[tid % WARPS];
@@ -624,6 +805,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
       const uint32_t v = __shfl_up_sync(0xffffffffu, it, o);
       if (lane >= o) it += v;
     }
+    const uint32_t total_ties = __shfl_sync(0xffffffffu, it, 31);
     uint32_t tie_at = it - nt;
     uint64_t m[PER], nm = 0;
     uint32_t tb[PER];
@@ -669,6 +851,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
       sh.pick_before = hits ? bhit : blst;
       sh.pick_ties = hits ? thit : tlst;
       sh.pick_total = W;
+      sh.pick_all_ties = total_ties;
     }
   }
   __syncthreads();
@@ -676,97 +859,89 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
   const uint64_t mine_before = sh.pick_before, W = sh.pick_total;
   const uint32_t my_tie_base = sh.pick_ties;
   const double want = u * (double)W;
-  if (target_warp == rank * WARPS + warp) {
+  // The block that has it: a thread per unit of that warp's part, in order.
+  if (target_warp / WARPS == rank) {
+    const int q0 = warp_begin(target_warp % WARPS), q1 = warp_begin(target_warp % WARPS + 1);
     uint64_t run = mine_before;
     uint32_t seen = my_tie_base;
-    int last = -1, token = -1;
-    double ylast = 0.0, ytoken = 0.0;
-    for (int qb = w0; qb < w1 && token < 0; qb += 32) {
-      const int q = qb + lane;
+    for (int qb = q0; qb < q1; qb += THREADS) {
+      const int q = qb + tid;
       float x[VEC];
       uint64_t f[VEC];
       double ys[VEC];
       uint32_t tie_bits = 0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        f[e] = 0;
-        x[e] = __uint_as_float(0x7fc00000u);
-        ys[e] = 0.0;
-      }
-      if (q < w1) un.load(q, x);
+      for (int e = 0; e < VEC; ++e) x[e] = __uint_as_float(0x7fc00000u);
+      if (q < q1) un.load(q, x);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        bool tie;
-        uint64_t v;
-        if (!kept(x[e], ys[e], v, tie)) continue;
-        f[e] = v;
-        if (tie) tie_bits |= 1u << e;
-      }
-      // ties of earlier lanes, then the ones that still stay
-      const uint32_t nt = __popc(tie_bits);
-      uint32_t it = nt;
+      for (int h = 0; h < VEC; h += 4) {
+        double y[4];
+        bool have[4];
+        uint64_t g[4];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, it, o);
-        if (lane >= o) it += v;
+        for (int e = 0; e < 4; ++e) {
+          bool tie;
+          have[e] = kept(x[h + e], ys[h + e], tie);
+          y[e] = have[e] ? ys[h + e] : 0.0;
+          if (have[e] && tie) tie_bits |= 1u << (h + e);
+        }
+        rw.fixed(y, have, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[h + e] = g[e];
       }
-      uint32_t at = seen + it - nt;
-      seen += __shfl_sync(0xffffffffu, it, 31);
+      unsigned long long pm, tm;
+      uint32_t pn, tn;
+      if (border.key != 0 && sh.pick_all_ties > border.ties) {
+        // of the tokens equal to the border only the first stay
+        scan(0, __popc(tie_bits), pm, pn, tm, tn);
+        pn += seen;
+        seen += tn;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (tie_bits >> e & 1) {
+            if (pn >= border.ties) f[e] = 0;
+            ++pn;
+          }
+      }
       uint64_t sum = 0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (tie_bits >> e & 1) {
-          if (at >= border.ties) f[e] = 0;
-          ++at;
-        }
-        sum += f[e];
-      }
-      uint64_t is = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t v = __shfl_up_sync(0xffffffffu, is, o);
-        if (lane >= o) is += v;
-      }
-      const uint64_t step = __shfl_sync(0xffffffffu, is, 31);
-      uint64_t acc = run + is - sum;
+      for (int e = 0; e < VEC; ++e) sum += f[e];
+      scan(sum, 0, pm, pn, tm, tn);
+      uint64_t acc = run + pm;
+      run += tm;
       int hit = -1, lst = -1;
       double yhit = 0.0, ylst = 0.0;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
+        if (f[e] == 0) continue;
         acc += f[e];
-        if (f[e] > 0) {
-          lst = q * VEC - un.shift + e;
-          ylst = ys[e];
-          if (hit < 0 && (double)acc > want) {
-            hit = lst;
-            yhit = ylst;
-          }
+        lst = q * VEC - un.shift + e;
+        ylst = ys[e];
+        if (hit < 0 && (double)acc > want) {
+          hit = lst;
+          yhit = ylst;
         }
       }
-      const uint32_t hits = __ballot_sync(0xffffffffu, hit >= 0);
-      if (hits) {
-        const int src = __ffs(hits) - 1;
-        token = __shfl_sync(0xffffffffu, hit, src);
-        ytoken = __shfl_sync(0xffffffffu, yhit, src);
+      // the first that passes u W: sums only grow, so it is the one whose
+      // predecessor does not
+      if (hit >= 0 && !((double)(acc - sum) > want)) {
+        sh.hit = hit;
+        sh.hit_y = yhit;
       }
       const uint32_t any = __ballot_sync(0xffffffffu, lst >= 0);
-      if (any) {
-        const int src = 31 - __clz(any);
-        last = __shfl_sync(0xffffffffu, lst, src);
-        ylast = __shfl_sync(0xffffffffu, ylst, src);
-      }
-      run += step;
+      if (any && lane == 31 - __clz(any)) atomicMax(&sh.last, lst);
+      __syncthreads();
+      if (lst >= 0 && lst == sh.last) sh.last_y = ylst;
+      __syncthreads();
+      if (sh.hit >= 0) break;
     }
-    if (token < 0) {  // u of 1 or more: the last kept token
-      token = last;
-      ytoken = ylast;
-    }
-    if (lane == 0) {
-      a.tokens[r] = token;
+    if (tid == 0) {
+      const bool have = sh.hit >= 0;  // u of 1 or more: the last kept token
+      a.tokens[r] = have ? sh.hit : sh.last;
       if (a.logprobs) {
         // log of (e / W) with e from its exponent: no digits of a small term are lost
         const double lw = log((double)W / a.scale);
-        a.logprobs[r] = (float)(-ytoken * 0.69314718055994530942 - lw);
+        a.logprobs[r] = (float)(-(have ? sh.hit_y : sh.last_y) * 0.69314718055994530942 - lw);
       }
     }
   }
@@ -774,7 +949,13 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(Args a) {
 }
 
 template <typename T>
-int run(const Args& a, int cluster, cudaStream_t st) {
+int run(const Args& a, cudaStream_t st) {
+  // Blocks of a row: as many as leave each at least 2048 tokens, while that leaves
+  // SMs idle; at least one for every 16384 tokens, so that a part stays in L1.
+  int cluster = 1;
+  while (cluster < MAX_CL && a.vocab > 16384 * cluster) cluster *= 2;
+  while (cluster < MAX_CL && a.rows * cluster * 2 <= sm_count() && a.vocab >= 2048 * 2 * cluster)
+    cluster *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * cluster));
   cfg.blockDim = dim3(THREADS);
@@ -828,13 +1009,8 @@ extern "C" int gq_sample(const void* logits, int dtype, int64_t rows, int64_t vo
   int log2v = 0;
   while ((1ll << log2v) < vocab) ++log2v;
   a.scale = (double)(1ll << std::min(45, 62 - log2v));
-  // A row is split over as many blocks as leave each at least 4096 logits and
-  // keep about two blocks per SM busy.
-  int cluster = 1;
-  while (cluster < samp::MAX_CL && rows * cluster * 2 <= 2 * sm_count() && vocab >= 4096 * 2 * cluster)
-    cluster *= 2;
   cudaStream_t st = as_stream(stream);
-  if (dtype == 0) return samp::run<float>(a, cluster, st);
-  if (dtype == 1) return samp::run<__nv_bfloat16>(a, cluster, st);
-  return samp::run<__half>(a, cluster, st);
+  if (dtype == 0) return samp::run<float>(a, st);
+  if (dtype == 1) return samp::run<__nv_bfloat16>(a, st);
+  return samp::run<__half>(a, st);
 }
