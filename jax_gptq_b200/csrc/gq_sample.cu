@@ -650,8 +650,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       z = warp_sum64(z);
       target = fmax(p, 0.0) * (double)z;
     }
-    int limit = -1;          // the bin down to which a border can lie
-    uint32_t through = 0;    // tokens down to there
+    // the bin down to which a border can lie that matters (min-p leaves nothing
+    // below its own), and the tokens down to there
+    int limit = -1;
+    uint32_t through = 0;
     if (cut_k) {
       limit = tell(bc < k && bc + hc >= k ? tid : -1, bc, 0, bc + hc, 0);
       through = sh.found_own;
@@ -664,6 +666,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       }
     }
     const uint32_t k_before = sh.found_count;  // with cut_k: tokens of the bins before
+    const int floor_bin = by_min ? (int)fmin(floor_y * 11.0 + 0.01, BINS - 2.0) : BINS - 2;
+    // (top-p after top-k needs the mass of all k, though)
+    if (limit > floor_bin && !(cut_k && by_p)) {
+      tell(tid == floor_bin ? tid : -1, 0, 0, bc + hc, 0);
+      // worth it where it makes the list short; the general way needs the border's own bin
+      if (sh.found_own <= LIST) {
+        limit = floor_bin;
+        through = sh.found_own;
+      }
+    }
     if (limit >= 0) {
       uint32_t n = LIST + 1;
       if (through <= LIST) {
@@ -678,7 +690,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       }
       if (n <= LIST) {
         sorted(n);
-        const uint32_t nk = cut_k ? min(k, n) : n;
+        const uint32_t nk = cut_k ? min(k, n) : n;  // (min-p may have made the list shorter than k)
         uint32_t place = nk - 1;
         if (by_p) {
           unsigned long long f[EACH], pm, total;
