@@ -19,8 +19,8 @@
 // uniform resolves.  Terms below 2^-(S+1) are zero: they can not be drawn.
 //
 // Split.  A cluster of up to 8 blocks takes a row, each a contiguous part, each
-// warp a contiguous part of that.  Passes over the row (from L1 and L2 after the
-// first):
+// warp a contiguous part of that, kept in shared memory (up to 131072 tokens in
+// float32; longer rows are read again from L1 and L2).  Passes over the row:
 //   1. the maximum;
 //   2. with top-k or top-p the number of tokens in 512 bins of log2 e (found in
 //      float32: any function that keeps the order will do); without top-k each
@@ -29,7 +29,7 @@
 //      first by which the sum is at least p (a bin's sum is at least its count
 //      times its smallest e).  Tokens down to there, where they are at most 2048,
 //      are collected and sorted by every block, and the borders read off their
-//      running sum.  Otherwise (flat distributions) top-k's border bin alone is
+//      running sum; up to 256 kept ones are drawn from right there.  Otherwise (flat distributions) top-k's border bin alone is
 //      sorted, then the sums of every bin are taken for top-p and its border bin
 //      is sorted; a bin of more than 2048 (runs of equal logits) is resolved by
 //      radix passes over the ordered bits;
@@ -45,6 +45,8 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 namespace cg = cooperative_groups;
 
@@ -56,6 +58,9 @@ constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 512;   // of log2 e, 11 to a power of two; one a thread
 constexpr int MAX_CL = 8;
 constexpr int LIST = 2048;  // tokens that are collected and sorted
+constexpr int RANKED = 256; // up to so many by counting, more by a sorting network
+constexpr int DIRECT = 256; // up to so many kept ones are drawn from without another pass
+constexpr int MAX_STAGE = 64 * 1024;  // bytes of a row that a block keeps in shared memory
 
 struct RowParam {  // a setting: one value, or one per row
   const void* rows;
@@ -174,21 +179,26 @@ struct Units {
     shift = (int)((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T));
     count = (v + shift + VEC - 1) / VEC;
   }
-  // NaN where there is no element
-  __device__ __forceinline__ void load(int q, float (&x)[VEC]) const {
+  // a unit's 16 bytes, NaN where there is no element
+  __device__ __forceinline__ uint4 load(int q) const {
     const int i0 = q * VEC - shift;
-    if (i0 >= 0 && i0 + VEC <= vocab) {
-      struct alignas(16) Pack { T e[VEC]; };
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + i0));
-      Pack p;
-      memcpy(&p, &raw, 16);
+    if (i0 >= 0 && i0 + VEC <= vocab) return __ldg(reinterpret_cast<const uint4*>(row + i0));
+    using Bits = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+    struct alignas(16) Pack { Bits e[VEC]; } p;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) x[e] = to_f<T>(p.e[e]);
-    } else {
+    for (int e = 0; e < VEC; ++e)
+      p.e[e] = (i0 + e >= 0 && i0 + e < vocab)
+                   ? reinterpret_cast<const Bits*>(row)[i0 + e]
+                   : (Bits)(sizeof(T) == 4 ? 0x7fc00000u : std::is_same<T, __half>::value ? 0x7e00u : 0x7fc0u);
+    uint4 raw;
+    memcpy(&raw, &p, 16);
+    return raw;
+  }
+  static __device__ __forceinline__ void values(const uint4& raw, float (&x)[VEC]) {
+    struct alignas(16) Pack { T e[VEC]; } p;
+    memcpy(&p, &raw, 16);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        x[e] = (i0 + e >= 0 && i0 + e < vocab) ? to_f<T>(row[i0 + e]) : __uint_as_float(0x7fc00000u);
-    }
+    for (int e = 0; e < VEC; ++e) x[e] = to_f<T>(p.e[e]);
   }
 };
 
@@ -207,14 +217,16 @@ struct Shared {
   unsigned long long mass[BINS];       // histogram over log2 e: sums
   uint32_t count[BINS];                // and tokens
   union {
-    uint32_t keys[LIST];               // collected from the whole row, sorted
+    alignas(16) unsigned long long keys[LIST];  // collected from the whole row, sorted
     struct {
       unsigned long long rmass[2][256];  // a radix pass, two buffers in turn
       uint32_t rcount[2][256];
     } radix;
   };
-  uint32_t list[LIST];                 // collected in this block
+  unsigned long long list[LIST];       // collected in this block
   uint32_t list_n, kmin, kmax;
+  unsigned long long term[DIRECT];     // a draw from the sorted list
+  uint32_t index[DIRECT];
   uint64_t wmass[WARPS];               // per warp: what the draw walks through
   uint32_t wties[WARPS];
   float mx[WARPS];
@@ -235,10 +247,12 @@ struct Shared {
   double hit_y, last_y;
 };
 
-template <typename T>
+// STAGED: the block's part of the row is kept in shared memory
+template <typename T, bool STAGED>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   constexpr int VEC = Units<T>::VEC;
   __shared__ Shared sh;
+  extern __shared__ uint4 stage[];
   cg::cluster_group cl = cg::this_cluster();
   const int CL = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -249,17 +263,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   const int b0 = (int)((int64_t)un.count * rank / CL), b1 = (int)((int64_t)un.count * (rank + 1) / CL);
   auto warp_begin = [&](int w) { return b0 + (int)((int64_t)(b1 - b0) * w / WARPS); };
   const int w0 = warp_begin(warp), w1 = warp_begin(warp + 1);
+  auto unit = [&](int q) { return STAGED ? stage[q - b0] : un.load(q); };
   // f(values, index of the first) for this lane's tokens, a unit at a time, NaN
-  // where there is none; the next unit is read ahead
+  // where there is none
   auto each_unit = [&](auto&& f) {
-    float x[VEC], next[VEC];
-    int q = w0 + lane;
-    if (q < w1) un.load(q, x);
-    for (; q < w1; q += 32) {
-      if (q + 32 < w1) un.load(q + 32, next);
+    for (int q = w0 + lane; q < w1; q += 32) {
+      float x[VEC];
+      un.values(unit(q), x);
       f(x, q * VEC - un.shift);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) x[e] = next[e];
     }
   };
   auto each_token = [&](auto&& f) {
@@ -280,12 +291,25 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   // ---- 1. the maximum (and for temperature 0 its first index)
   float mx = -INFINITY;
   uint32_t arg = 0xffffffffu;
-  each_token([&](float x, int i) {
-    if (x > mx) {  // indices grow along a lane's walk: the first one stays
-      mx = x;
-      arg = (uint32_t)i;
+  for (int q = w0 + lane; q < w1; q += 128) {  // four units in flight
+    uint4 raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (q + 32 * i < w1) raw[i] = un.load(q + 32 * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (q + 32 * i >= w1) break;
+      if (STAGED) stage[q + 32 * i - b0] = raw[i];
+      float x[VEC];
+      un.values(raw[i], x);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (x[e] > mx) {  // indices grow along a lane's walk: the first one stays
+          mx = x[e];
+          arg = (uint32_t)((q + 32 * i) * VEC - un.shift + e);
+        }
     }
-  });
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float om = __shfl_xor_sync(0xffffffffu, mx, o);
@@ -303,8 +327,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   sh.count[tid] = 0;
   if (tid == 0) {
     sh.list_n = 0;
-    sh.kmin = 0xffffffffu;
-    sh.kmax = 0;
     sh.hit = sh.last = -1;
   }
   __syncthreads();
@@ -461,42 +483,36 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     while (j < own && (double)(msum + (unsigned long long)j * each) < target) ++j;
     return j;
   };
-  // Collects the keys of this row's tokens that `pred` picks; the number of them
-  // over the whole row, of which the first LIST are in this block's `list`s.
+  // Collects this row's tokens that `pred` picks, as (bits in order, ~index): larger
+  // is earlier.  The number of them over the whole row; if that is at most LIST they
+  // are in the blocks' `list`s, block c's ending at `upto` of lane c.
+  uint32_t upto = 0;
   auto collect = [&](auto&& pred) {
     __syncthreads();
-    if (tid == 0) {
-      sh.list_n = 0;
-      sh.kmin = 0xffffffffu;
-      sh.kmax = 0;
-    }
+    if (tid == 0) sh.list_n = 0;
     __syncthreads();
-    each_token([&](float x, int) {
+    each_token([&](float x, int i) {
       if (!pred(x)) return;
-      const uint32_t key = ordered(x);
       const uint32_t at = atomicAdd(&sh.list_n, 1u);
-      if (at < LIST) sh.list[at] = key;
-      atomicMin(&sh.kmin, key);
-      atomicMax(&sh.kmax, key);
+      if (at < LIST) sh.list[at] = (unsigned long long)ordered(x) << 32 | ~(uint32_t)i;
     });
     cl.sync();
-    const uint32_t n = __reduce_add_sync(0xffffffffu, lane < CL ? peer(lane)->list_n : 0);
-    if (n > LIST) cl.sync();  // the lists are not read further and may be begun anew
-    return n;
-  };
-  // The collected keys (n <= LIST) of all blocks in `keys`, largest first.
-  auto sorted = [&](uint32_t n) {
-    const uint32_t mine = lane < CL ? peer(lane)->list_n : 0;
-    uint32_t upto = mine;
+    upto = lane < CL ? peer(lane)->list_n : 0;
 #pragma unroll
     for (int o = 1; o < MAX_CL; o <<= 1) {
       const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
+    const uint32_t n = __shfl_sync(0xffffffffu, upto, MAX_CL - 1);
+    if (n > LIST) cl.sync();  // the lists are not read further and may be begun anew
+    return n;
+  };
+  // The n <= LIST collected tokens of all blocks in `keys`, the earliest first.
+  auto sorted = [&](uint32_t n) {
     uint32_t size = 64;
     while (size < n) size *= 2;
     for (uint32_t i = tid; i < ((size + 31) & ~31u); i += THREADS) {
-      uint32_t key = 0;  // below every key
+      unsigned long long key = 0;  // below every token
       uint32_t c = 0, from = 0;
 #pragma unroll
       for (int o = 0; o < MAX_CL; ++o) {
@@ -509,6 +525,22 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       if (i < n) key = peer(c)->list[i - from];
       if (i < size) sh.keys[i] = key;
     }
+    if (n <= RANKED) {
+      __syncthreads();
+      unsigned long long key = 0;
+      uint32_t at = 0;
+      if (tid < n) {
+        key = sh.keys[tid];
+        for (uint32_t j = 0; j < n; j += 2) {  // (an odd last one meets a 0)
+          const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.keys[j]);
+          at += (o.x > key) + (o.y > key);
+        }
+      }
+      __syncthreads();
+      if (tid < n) sh.keys[at] = key;
+      __syncthreads();
+      return;
+    }
     // bitonic network; pairs up to 32 apart stay inside a warp's 64 keys
     uint32_t last = 64;
     for (uint32_t k2 = 2; k2 <= size; k2 *= 2)
@@ -518,7 +550,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
         last = j;
         for (uint32_t t = tid; t < size / 2; t += THREADS) {
           const uint32_t i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
-          const uint32_t x = sh.keys[i], y = sh.keys[i + j];
+          const unsigned long long x = sh.keys[i], y = sh.keys[i + j];
           if (((i & k2) == 0) == (x < y)) {
             sh.keys[i] = y;
             sh.keys[i + j] = x;
@@ -527,39 +559,40 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       }
     __syncthreads();
   };
-  // The terms of the first n sorted keys, EACH a thread, with their running sum; and
-  // the number of the last one that begins before `target` (at least the first).
+  auto sorted_value = [&](uint32_t i) { return from_ordered((uint32_t)(sh.keys[i] >> 32)); };
+  // The terms of the first n sorted tokens, EACH a thread, with their running sum;
+  // and the number of the last one that begins before `target` (at least the first).
   constexpr int EACH = LIST / THREADS;
-  auto running = [&](uint32_t n, unsigned long long (&f)[EACH], unsigned long long& pm,
+  auto running = [&](uint32_t n, uint64_t (&f)[EACH], unsigned long long& pm,
                      unsigned long long& total) {
+    double y[EACH];
+    bool have[EACH];
 #pragma unroll
     for (int h = 0; h < EACH; ++h) {
-      const uint32_t i = EACH * tid + h;
-      f[h] = i < n ? rw.fixed(from_ordered(sh.keys[i])) : 0;
+      have[h] = EACH * tid + h < n && rw.distance(sorted_value(EACH * tid + h), y[h]);
+      y[h] = have[h] ? y[h] : 0.0;
     }
+    rw.fixed(y, have, f);
     uint32_t pn, tn;
     scan(f[0] + f[1] + f[2] + f[3], 0, pm, pn, total, tn);
   };
-  auto last_before = [&](uint32_t n, const unsigned long long (&f)[EACH], unsigned long long pm,
-                         double target) {
-    uint32_t stays = 0;
+  auto last_before = [&](uint32_t n, const uint64_t (&f)[EACH], unsigned long long pm, double target) {
+    int mine = -1;
 #pragma unroll
     for (int h = 0; h < EACH; ++h) {
-      if (EACH * tid + h < n && (double)pm < target) ++stays;
+      const bool stays = EACH * tid + h < n && (double)pm < target;
       pm += f[h];
+      if (stays && !(EACH * tid + h + 1 < n && (double)pm < target)) mine = EACH * tid + h;
     }
-    unsigned long long qm, tm;
-    uint32_t pn, tn;
-    scan(0, stays, qm, pn, tm, tn);
-    return max(tn, 1u) - 1;
+    return (uint32_t)max(tell(mine, 0, 0, 0, 0), 0);
   };
-  auto border_at = [&](uint32_t place, Border& out) {  // after sorted key number `place`
-    out.key = sh.keys[place];
-    uint32_t ties = 0;
-    for (uint32_t i = tid; i <= place; i += THREADS) ties += sh.keys[i] == out.key;
-    unsigned long long pm, tm;
-    uint32_t pn;
-    scan(0, ties, pm, pn, tm, out.ties);
+  auto border_at = [&](uint32_t place, Border& out) {  // after sorted token number `place`
+    out.key = (uint32_t)(sh.keys[place] >> 32);
+    int first = -1;  // of the equal ones
+    for (uint32_t i = tid; i <= place; i += THREADS)
+      if ((uint32_t)(sh.keys[i] >> 32) == out.key && (i == 0 || (uint32_t)(sh.keys[i - 1] >> 32) != out.key))
+        first = (int)i;
+    out.ties = place - (uint32_t)tell(first, 0, 0, 0, 0) + 1;
   };
   static_assert(EACH == 4, "sums of four");
   // Radix passes over the members of bin `fb` with keys above `above`, before which
@@ -568,9 +601,26 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   // `k` tokens do.
   auto radix = [&](bool by_mass, int fb, uint32_t above, uint32_t cnt, unsigned long long msum,
                    double target, Border& out) {
-    uint32_t lo = lane < CL ? peer(lane)->kmin : 0xffffffffu, hi = lane < CL ? peer(lane)->kmax : 0u;
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
+    __syncthreads();
+    if (tid == 0) {
+      sh.kmin = 0xffffffffu;
+      sh.kmax = 0;
+    }
+    __syncthreads();
+    uint32_t lo = 0xffffffffu, hi = 0;
+    each_token([&](float x, int) {
+      if (bin_of(x) != fb) return;
+      const uint32_t key = ordered(x);
+      if (key <= above) return;
+      lo = min(lo, key);
+      hi = max(hi, key);
+    });
+    atomicMin(&sh.kmin, lo);
+    atomicMax(&sh.kmax, hi);
+    cl.sync();
+    lo = __reduce_min_sync(0xffffffffu, lane < CL ? peer(lane)->kmin : 0xffffffffu);
+    hi = __reduce_max_sync(0xffffffffu, lane < CL ? peer(lane)->kmax : 0u);
+    cl.sync();  // all have read them
     int bits = 32 - __clz(lo ^ hi), buf = 0;
     uint32_t prefix = bits >= 32 ? 0 : (hi >> bits) << bits;
     uint32_t own = 0;               // tokens equal to the key so far
@@ -627,6 +677,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     out.ties = by_mass ? staying(own, own ? own_mass / own : 0, msum, target) : min(own, k - cnt);
   };
 
+  int direct = -1;  // the kept tokens are the sorted list up to this one
   if (by_k || by_p) {
     // this thread's bin over the whole row: tokens, and the least that its sum can be
     // (count * 2^-((bin + 1) / 11), with room for roundings)
@@ -693,12 +744,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
         const uint32_t nk = cut_k ? min(k, n) : n;  // (min-p may have made the list shorter than k)
         uint32_t place = nk - 1;
         if (by_p) {
-          unsigned long long f[EACH], pm, total;
+          uint64_t f[EACH];
+          unsigned long long pm, total;
           running(nk, f, pm, total);
           if (cut_k) target = fmax(p, 0.0) * (double)total;
           place = last_before(nk, f, pm, target);
         }
-        border_at(place, border);
+        if (place < DIRECT) {
+          direct = (int)place;
+        } else {
+          border_at(place, border);
+        }
       } else {
         if (cut_k) {
           n = collect([&](float x) { return bin_of(x) == limit; });
@@ -710,10 +766,27 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
           }
         }
         if (by_p) {
-          each_token([&](float x, int) {
-            const int b = bin_of(x);
-            if (b <= limit && (!cut_k || ordered(x) > border.key))
-              atomicAdd(&sh.mass[b], (unsigned long long)rw.fixed(x));
+          each_unit([&](const float (&x)[VEC], int) {
+#pragma unroll
+            for (int h = 0; h < VEC; h += 4) {
+              double y[4];
+              bool have[4], any = false;
+              int b[4];
+              uint64_t f[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                b[e] = bin_of(x[h + e]);
+                have[e] = b[e] <= limit && (!cut_k || ordered(x[h + e]) > border.key) &&
+                          rw.distance(x[h + e], y[e]);
+                y[e] = have[e] ? y[e] : 0.0;
+                any |= have[e];
+              }
+              if (!any) continue;
+              rw.fixed(y, have, f);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (have[e]) atomicAdd(&sh.mass[b[e]], (unsigned long long)f[e]);
+            }
           });
           cl.sync();
           unsigned long long hm = 0, pm;
@@ -732,7 +805,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
             n = collect([&](float x) { return bin_of(x) == fb && ordered(x) > above; });
             if (n <= LIST) {
               sorted(n);
-              unsigned long long f[EACH], total;
+              uint64_t f[EACH];
+              unsigned long long total;
               running(n, f, pm, total);
               border_at(last_before(n, f, pm + msum, target), border);
             } else {
@@ -745,7 +819,50 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       }
     }
     // p = 0, or sums that leave the first token alone
-    if (by_p && !(target > 0.0)) border = Border{ordered(mx), 1};
+    if (by_p && !(target > 0.0)) {
+      border = Border{ordered(mx), 1};
+      direct = -1;
+    }
+  }
+
+  // A short list of kept tokens is all that the draw needs: block 0 adds up, for
+  // each of them, the terms of those with a smaller index.
+  if (direct >= 0) {
+    if (rank == 0) {
+      const uint32_t n = (uint32_t)direct + 1;
+      double y = 0.0;
+      uint32_t index = 0;
+      uint64_t f = 0;
+      if (tid < n) {
+        const float x = sorted_value(tid);
+        index = ~(uint32_t)sh.keys[tid];
+        if (rw.distance(x, y) && !(by_min && y > floor_y)) f = rw.fixed(x);
+      }
+      if (tid < DIRECT) {
+        sh.term[tid] = f;
+        sh.index[tid] = index;
+      }
+      __syncthreads();
+      uint64_t before = 0, W = 0;
+      uint32_t latest = 0;
+      for (uint32_t j = 0; j < n; ++j) {
+        const uint64_t t = sh.term[j];
+        const uint32_t o = sh.index[j];
+        W += t;
+        before += o < index ? t : 0;
+        if (t > 0) latest = max(latest, o);
+      }
+      const double want = u * (double)W;
+      // the one that passes u W, or for u of 1 or more the last
+      const bool passes = (before == 0 || !((double)before > want)) && (double)(before + f) > want;
+      if (f > 0 && (passes || (index == latest && !((double)W > want)))) {
+        a.tokens[r] = index;
+        if (a.logprobs)
+          a.logprobs[r] = (float)(-y * 0.69314718055994530942 - log((double)W / a.scale));
+      }
+    }
+    cl.sync();  // no block leaves while another may read its shared memory
+    return;
   }
 
   // ---- 4. what is kept, per warp
@@ -884,7 +1001,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       uint32_t tie_bits = 0;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) x[e] = __uint_as_float(0x7fc00000u);
-      if (q < q1) un.load(q, x);
+      if (q < q1) un.values(unit(q), x);
 #pragma unroll
       for (int h = 0; h < VEC; h += 4) {
         double y[4];
@@ -936,7 +1053,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       }
       // the first that passes u W: sums only grow, so it is the one whose
       // predecessor does not
-      if (hit >= 0 && !((double)(acc - sum) > want)) {
+      if (hit >= 0 && (acc == sum || !((double)(acc - sum) > want))) {
         sh.hit = hit;
         sh.hit_y = yhit;
       }
@@ -963,7 +1080,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
 template <typename T>
 int run(const Args& a, cudaStream_t st) {
   // Blocks of a row: as many as leave each at least 2048 tokens, while that leaves
-  // SMs idle; at least one for every 16384 tokens, so that a part stays in L1.
+  // SMs idle; at least one for every 16384 tokens, so that a part fits shared memory.
   int cluster = 1;
   while (cluster < MAX_CL && a.vocab > 16384 * cluster) cluster *= 2;
   while (cluster < MAX_CL && a.rows * cluster * 2 <= sm_count() && a.vocab >= 2048 * 2 * cluster)
@@ -977,7 +1094,24 @@ int run(const Args& a, cudaStream_t st) {
   at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, a);
+  // a block's part of the row, in units of 16 bytes (one more where they do not divide)
+  const int64_t part = (ceil_div(ceil_div(a.vocab, (int64_t)(16 / sizeof(T))) + 1, cluster) + 1) * 16;
+  cudaError_t e;
+  if (part <= MAX_STAGE + 256) {
+    static std::atomic<uint64_t> ready{0};  // devices on which the attribute is set
+    int dev = 0;
+    GQ_CHECK_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev > 63 || !(ready.load(std::memory_order_acquire) & bit)) {
+      GQ_CHECK_CUDA(cudaFuncSetAttribute(sample_kernel<T, true>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_STAGE + 256));
+      ready.fetch_or(bit, std::memory_order_release);
+    }
+    cfg.dynamicSmemBytes = (size_t)part;
+    e = cudaLaunchKernelEx(&cfg, sample_kernel<T, true>, a);
+  } else {
+    e = cudaLaunchKernelEx(&cfg, sample_kernel<T, false>, a);
+  }
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(GQ_ECUDA, "gq_sample: %s", cudaGetErrorString(e));
