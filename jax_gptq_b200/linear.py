@@ -143,7 +143,7 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
         x2 = x.reshape(-1, n).contiguous()
     tokens, ldx = x2.shape[0], x2.stride(0)
     if out is None:
-        out = x.new_empty((tokens, m) if x2 is x else (*x.shape[:-1], m))
+        out = x.new_empty(tokens, m) if x2 is x else x.new_empty(*x.shape[:-1], m)
     elif tuple(out.shape) != (*x.shape[:-1], m) or out.dtype != x.dtype or \
             out.device != x.device or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {x.dtype} tensor {(*x.shape[:-1], m)} on "

@@ -8,8 +8,8 @@ the frequencies only (and for :class:`YarnScaling` a factor on the result).
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from dataclasses import dataclass
 from fractions import Fraction
 
@@ -20,7 +20,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _POSITIONS = (torch.int64, torch.int32)
-_STRIDES = ctypes.c_int64 * 12
+_STRIDES = struct.Struct("12q").pack  # the strides argument of gq_rotary
 _PI = Fraction("3.14159265358979323846264338327950288419716939937510")
 
 
@@ -181,21 +181,24 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     dt = _DTYPES.get(q.dtype)
     if dt is None:
         raise ValueError(f"q must be float32, bfloat16 or float16, got {q.dtype}")
-    q = _heads("q", q, plan)
+    if q.dim() != 4 or q.stride(3) != 1 or q.shape[3] != plan.head_dim:
+        q = _heads("q", q, plan)
     b, h, s, d = q.shape
     hk = 0
     if k is not None:
-        if k.dtype != q.dtype or k.device != q.device:
+        if k.dtype != q.dtype or k.get_device() != q.get_device():
             raise ValueError("q and k must have one type and device")
-        k = _heads("k", k, plan)
+        if k.dim() != 4 or k.stride(3) != 1 or k.shape[3] != d:
+            k = _heads("k", k, plan)
         kb, hk, ks, _ = k.shape
         if kb != b or ks != s:
             raise ValueError(f"q and k must have one batch and length, got {tuple(q.shape)} and "
                              f"{tuple(k.shape)}")
-    pshape = tuple(positions.shape)
-    if positions.dtype not in _POSITIONS or (pshape != (s,) and pshape != (b, s)):
+    pdim = positions.dim()
+    if positions.dtype not in _POSITIONS or not 1 <= pdim <= 2 or positions.shape[-1] != s or \
+            (pdim == 2 and positions.shape[0] != b):
         raise ValueError(f"positions must be int64 or int32 [{s}] or [{b}, {s}], got "
-                         f"{positions.dtype} {pshape}")
+                         f"{positions.dtype} {tuple(positions.shape)}")
     dev = q.get_device()
     if dev < 0 or positions.get_device() != dev or plan.turns.get_device() != dev:
         raise ValueError(f"q, positions and the plan must be on one CUDA device, got {q.device}, "
@@ -211,17 +214,19 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         oq, ok = _results(q, k, out)
     if b == 0 or s == 0 or h + hk == 0:
         return oq, ok
-    qs, qos = q.stride(), oq.stride()
+    q0, q1, q2, _ = q.stride()
+    o0, o1, o2, _ = oq.stride()
     if hk:
-        kst, kos = k.stride(), ok.stride()
-        st = _STRIDES(*qs[:3], *qos[:3], *kst[:3], *kos[:3])
+        k0, k1, k2, _ = k.stride()
+        p0, p1, p2, _ = ok.stride()
+        strides = _STRIDES(q0, q1, q2, o0, o1, o2, k0, k1, k2, p0, p1, p2)
         kp, kop = k.data_ptr(), ok.data_ptr()
     else:
-        st = _STRIDES(*qs[:3], *qos[:3])
+        strides = _STRIDES(q0, q1, q2, o0, o1, o2, 0, 0, 0, 0, 0, 0)
         kp = kop = None
     status = _lib.lib().gq_rotary(
-        q.data_ptr(), oq.data_ptr(), h, kp, kop, hk, st, positions.data_ptr(),
-        positions.stride(0) if len(pshape) == 2 else 0, positions.dtype is torch.int32,
+        q.data_ptr(), oq.data_ptr(), h, kp, kop, hk, strides, positions.data_ptr(),
+        positions.stride(0) if pdim == 2 else 0, positions.dtype is torch.int32,
         plan.turns.data_ptr(), b, s, d, plan.rotary_dim, plan.interleaved, plan.factor, transpose,
         dt, A.raw_stream(dev))
     if status:

@@ -72,13 +72,16 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return sample_tokens(logits, u, temperature, top_k, top_p, min_p)
-    up, uk, _, ut = _setting("u", u.reshape(1) if u.dim() == 0 else u, rows, lg, 0.0, None)
+    uk = _KINDS[u.dtype]
+    if u.dim() != 1 or u.shape[0] != rows or u.get_device() != dev or u.stride(0) != 1:
+        up, uk, _, u = _setting("u", u.reshape(1) if u.dim() == 0 else u, rows, lg, 0.0, None)
+    up = u.data_ptr()
     tp, tk, tv, t0 = _setting("temperature", temperature, rows, lg, 0.0, None)
     kp, kk, kv, t1 = _setting("top_k", top_k, rows, lg, 0, None)
     pp, pk, pv, t2 = _setting("top_p", top_p, rows, lg, 0.0, 1.0)
     mp, mk, mv, t3 = _setting("min_p", min_p, rows, lg, 0.0, 1.0)
-    tokens = lg.new_empty((rows,), dtype=torch.int64)
-    logprobs = lg.new_empty((rows,), dtype=torch.float32)
+    tokens = torch.empty_like(u, dtype=torch.int64)
+    logprobs = torch.empty_like(u, dtype=torch.float32)
     if rows:
         status = _lib.lib().gq_sample(lg.data_ptr(), dt, rows, vocab, lg.stride(0), up, uk, tp, tk,
                                       tv, kp, kk, kv, pp, pk, pv, mp, mk, mv, tokens.data_ptr(),
