@@ -29,10 +29,13 @@
 //      first by which the sum is at least p (a bin's sum is at least its count
 //      times its smallest e).  Tokens down to there, where they are at most 2048,
 //      are collected and sorted by every block, and the borders read off their
-//      running sum; up to 256 kept ones are drawn from right there.  Otherwise (flat distributions) top-k's border bin alone is
-//      sorted, then the sums of every bin are taken for top-p and its border bin
-//      is sorted; a bin of more than 2048 (runs of equal logits) is resolved by
-//      radix passes over the ordered bits;
+//      running sum; up to 256 kept ones are drawn from right there.
+//      Otherwise (flat distributions) top-k's border bin alone is sorted; for top-p
+//      the counts also tell from which bin on the border can lie (a bin's sum is at
+//      most its count times its largest e), one pass adds up what lies before and
+//      512 cells between the two, and the border's cell is sorted.  More than 2048
+//      tokens in one (runs of equal logits) are resolved by radix passes over the
+//      ordered bits;
 //   4. with filters each warp's sum of the kept e and its number of tokens equal
 //      to the border;
 //   5. the block that holds u W finds the token in the part of one warp.
@@ -47,6 +50,7 @@
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
+#include <utility>
 
 namespace cg = cooperative_groups;
 
@@ -58,7 +62,7 @@ constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 512;   // of log2 e, 11 to a power of two; one a thread
 constexpr int MAX_CL = 8;
 constexpr int LIST = 2048;  // tokens that are collected and sorted
-constexpr int RANKED = 256; // up to so many by counting, more by a sorting network
+constexpr int RANKED = 512; // up to so many by counting, more by a sorting network
 constexpr int DIRECT = 256; // up to so many kept ones are drawn from without another pass
 constexpr int MAX_STAGE = 64 * 1024;  // bytes of a row that a block keeps in shared memory
 
@@ -86,6 +90,7 @@ struct Args {
   int64_t* tokens;
   float* logprobs;
   double scale;  // 2^S
+  int limb;      // bits: 3 limbs hold a term, and 32 bits the sum of a block's
 };
 
 template <typename T>
@@ -214,8 +219,8 @@ struct Border {
 };
 
 struct Shared {
-  unsigned long long mass[BINS];       // histogram over log2 e: sums
-  uint32_t count[BINS];                // and tokens
+  uint32_t count[BINS];                // histogram over log2 e: tokens
+  uint32_t mass[3][BINS];              // and sums, by limbs of a.limb bits
   union {
     alignas(16) unsigned long long keys[LIST];  // collected from the whole row, sorted
     struct {
@@ -323,8 +328,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     sh.mx[warp] = mx;
     sh.amax[warp] = arg;
   }
-  sh.mass[tid] = 0;
-  sh.count[tid] = 0;
+  sh.count[tid] = sh.mass[0][tid] = sh.mass[1][tid] = sh.mass[2][tid] = 0;
   if (tid == 0) {
     sh.list_n = 0;
     sh.hit = sh.last = -1;
@@ -378,10 +382,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   const float cf = (float)fmin(rw.c, 3e38);
   // bin of a token; the last bin holds only terms that are zero (46.45 powers of
   // two below the largest and further), and whatever is no token at all
-  auto bin_of = [&](float l) {
+  auto depth = [&](float l) {  // in bins
     const float y = l == mx ? 0.f : (mx - l) * cf;
-    return min(BINS - 1, (int)(fminf(y, 50.f) * 11.f));
+    return fminf(y, 50.f) * 11.f;
   };
+  auto bin_of = [&](float l) { return min(BINS - 1, (int)depth(l)); };
   const bool by_k = kd >= 1.0 && kd < (double)a.vocab;
   const uint32_t k = by_k ? (uint32_t)kd : 0;
   const bool by_p = p < 1.0;
@@ -595,12 +600,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     out.ties = place - (uint32_t)tell(first, 0, 0, 0, 0) + 1;
   };
   static_assert(EACH == 4, "sums of four");
-  // Radix passes over the members of bin `fb` with keys above `above`, before which
-  // `cnt` tokens of mass `msum` lie, with digits of 8 bits from the highest bit in
+  // Radix passes over the tokens that `member` picks (neighbours in value), before
+  // which `cnt` tokens of mass `msum` lie, with digits of 8 bits from the highest bit in
   // which they differ.  by_mass: the tokens that begin before `target` stay; else
   // `k` tokens do.
-  auto radix = [&](bool by_mass, int fb, uint32_t above, uint32_t cnt, unsigned long long msum,
-                   double target, Border& out) {
+  auto radix = [&](auto&& member, bool by_mass, uint32_t cnt, unsigned long long msum, double target,
+                   Border& out) {
     __syncthreads();
     if (tid == 0) {
       sh.kmin = 0xffffffffu;
@@ -609,9 +614,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     __syncthreads();
     uint32_t lo = 0xffffffffu, hi = 0;
     each_token([&](float x, int) {
-      if (bin_of(x) != fb) return;
+      if (!member(x)) return;
       const uint32_t key = ordered(x);
-      if (key <= above) return;
       lo = min(lo, key);
       hi = max(hi, key);
     });
@@ -637,9 +641,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       const uint32_t dmask = bits > 0 ? ((bits >= 32 ? 0xffffffffu : (1u << bits) - 1u) >> shift) : 0u;
       const uint32_t high = bits >= 32 ? 0u : ~((1u << bits) - 1u);
       each_token([&](float x, int) {
-        if (bin_of(x) != fb) return;
+        if (!member(x)) return;
         const uint32_t key = ordered(x);
-        if (key <= above || (key & high) != (prefix & high)) return;
+        if ((key & high) != (prefix & high)) return;
         const uint32_t d = dmask - ((key >> shift) & dmask);  // largest first
         atomicAdd(&sh.radix.rcount[buf][d], 1u);
         if (by_mass) atomicAdd(&sh.radix.rmass[buf][d], (unsigned long long)rw.fixed(x));
@@ -697,8 +701,15 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     unsigned long long z = 0;  // mass that top-k leaves
     double target = 0.0;
     if (by_p && !cut_k) {
-      for (int i = lane; i < CL * WARPS; i += 32) z += peer(i / WARPS)->wmass[i % WARPS];
-      z = warp_sum64(z);
+      if (warp == 0) {
+#pragma unroll
+        for (int i = 0; i < MAX_CL * WARPS / 32; ++i)
+          if (32 * i + lane < CL * WARPS)
+            z += peer((32 * i + lane) / WARPS)->wmass[(32 * i + lane) % WARPS];
+        z = warp_sum64(z);
+      }
+      tell(tid == 0 ? 0 : -1, 0, z, 0, 0);
+      z = sh.found_mass;
       target = fmax(p, 0.0) * (double)z;
     }
     // the bin down to which a border can lie that matters (min-p leaves nothing
@@ -762,47 +773,100 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
             sorted(n);
             border_at(k - k_before - 1, border);
           } else {
-            radix(false, limit, 0u, k_before, 0, 0.0, border);
+            radix([&](float x) { return bin_of(x) == limit; }, false, k_before, 0, 0.0, border);
           }
         }
         if (by_p) {
+          const uint32_t above = cut_k ? border.key : 0u;
+          const unsigned long long each = cut_k ? rw.fixed(from_ordered(border.key)) : 0;
+          auto add_up = [&](uint64_t mine) {  // over the row
+            mine = warp_sum64(mine);
+            if (lane == 0) sh.wmass[warp] = mine;
+            cl.sync();
+            unsigned long long all = 0;
+            if (warp == 0) {
+#pragma unroll
+              for (int i = 0; i < MAX_CL * WARPS / 32; ++i)
+                if (32 * i + lane < CL * WARPS)
+                  all += peer((32 * i + lane) / WARPS)->wmass[(32 * i + lane) % WARPS];
+              all = warp_sum64(all);
+            }
+            tell(tid == 0 ? 0 : -1, 0, all, 0, 0);
+            return sh.found_mass;
+          };
+          if (cut_k) {  // what top-k left
+            uint64_t mine = 0;
+            each_token([&](float x, int) {
+              if (x > -INFINITY && ordered(x) > above) mine += rw.fixed(x);
+            });
+            target = fmax(p, 0.0) * (double)(add_up(mine) + border.ties * each);
+          }
+          cl.sync();  // wmass is read and may be written again
+          // the first bin by whose end the sum can have reached the target: a bin's sum
+          // is at most its count times its largest e
+          const unsigned long long most = (unsigned long long)(
+              hc * (double)exp2f(-((float)tid - 0.01f) / 11.f) * 1.0001 * rw.scale) + hc;
+          unsigned long long pm;
+          uint32_t pn, tn;
+          scan(most, 0, pm, pn, tm, tn);
+          const int low =
+              max(tell((double)pm < target && !((double)(pm + most) < target) ? tid : -1, 0, 0, 0, 0), 0);
+          // one pass: the sum of what lies before bin `low`, and of each of 512 cells
+          // between there and bin `limit`
+          const float split = (float)max(1, BINS / max(1, limit + 1 - min(low, limit)));
+          const float first_depth = (float)min(low, limit), end_depth = (float)(limit + 1);
+          auto cell = [&](float x) {  // -1 before, BINS behind
+            const float d = depth(x);
+            if (!(d < end_depth) || (cut_k && ordered(x) <= above)) return BINS;
+            return d < first_depth ? -1 : min(BINS - 1, (int)((d - first_depth) * split));
+          };
+          uint64_t before = 0;
           each_unit([&](const float (&x)[VEC], int) {
 #pragma unroll
             for (int h = 0; h < VEC; h += 4) {
               double y[4];
-              bool have[4], any = false;
-              int b[4];
+              bool have[4];
+              int c[4];
               uint64_t f[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                b[e] = bin_of(x[h + e]);
-                have[e] = b[e] <= limit && (!cut_k || ordered(x[h + e]) > border.key) &&
-                          rw.distance(x[h + e], y[e]);
+                c[e] = cell(x[h + e]);
+                have[e] = c[e] < BINS && rw.distance(x[h + e], y[e]);
                 y[e] = have[e] ? y[e] : 0.0;
-                any |= have[e];
               }
-              if (!any) continue;
+              if (!(have[0] || have[1] || have[2] || have[3])) continue;
               rw.fixed(y, have, f);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (have[e]) atomicAdd(&sh.mass[b[e]], (unsigned long long)f[e]);
+              for (int e = 0; e < 4; ++e) {
+                if (!have[e]) continue;
+                if (c[e] < 0) {
+                  before += f[e];
+                } else {  // (64-bit additions here took 5 times as long)
+                  const uint32_t mask = (1u << a.limb) - 1u;
+                  atomicAdd(&sh.mass[0][c[e]], (uint32_t)f[e] & mask);
+                  atomicAdd(&sh.mass[1][c[e]], (uint32_t)(f[e] >> a.limb) & mask);
+                  atomicAdd(&sh.mass[2][c[e]], (uint32_t)(f[e] >> 2 * a.limb));
+                }
+              }
             }
           });
-          cl.sync();
-          unsigned long long hm = 0, pm;
-          uint32_t pn, tn;
+          const unsigned long long base = add_up(before);
+          unsigned long long hm = 0;
 #pragma unroll
           for (int c = 0; c < MAX_CL; ++c)
-            if (c < CL) hm += peer(c)->mass[tid];
+            if (c < CL) {
+              const Shared* o = peer(c);
+              hm += o->mass[0][tid] + ((unsigned long long)o->mass[1][tid] << a.limb) +
+                    ((unsigned long long)o->mass[2][tid] << 2 * a.limb);
+            }
           scan(hm, 0, pm, pn, tm, tn);
-          const unsigned long long each = cut_k ? rw.fixed(from_ordered(border.key)) : 0;
-          if (cut_k) target = fmax(p, 0.0) * (double)(tm + border.ties * each);
-          // the last bin that begins before the target
-          const int fb = tell((double)pm < target && !((double)(pm + hm) < target) ? tid : -1, 0, pm, 0, 0);
+          pm += base;
+          // the last cell that begins before the target
+          const int fc = tell((double)pm < target && !((double)(pm + hm) < target) ? tid : -1, 0, pm, 0, 0);
           const unsigned long long msum = sh.found_mass;
-          if (fb >= 0) {
-            const uint32_t above = cut_k ? border.key : 0u;
-            n = collect([&](float x) { return bin_of(x) == fb && ordered(x) > above; });
+          if (fc >= 0) {
+            auto member = [&](float x) { return cell(x) == fc; };
+            n = collect(member);
             if (n <= LIST) {
               sorted(n);
               uint64_t f[EACH];
@@ -810,10 +874,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
               running(n, f, pm, total);
               border_at(last_before(n, f, pm + msum, target), border);
             } else {
-              radix(true, fb, above, 0, msum, target, border);
+              radix(member, true, 0, msum, target, border);
             }
-          } else if (cut_k) {  // among the tokens equal to top-k's border
-            border.ties = staying(border.ties, each, tm, target);
+          } else {
+            if (cut_k) border.ties = staying(border.ties, each, base + tm, target);  // among equal ones
+            cl.sync();  // as above
           }
         }
       }
@@ -828,6 +893,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   // A short list of kept tokens is all that the draw needs: block 0 adds up, for
   // each of them, the terms of those with a smaller index.
   if (direct >= 0) {
+    // nothing more is read from another block: one may leave when all are here
+    auto here = cl.barrier_arrive();
     if (rank == 0) {
       const uint32_t n = (uint32_t)direct + 1;
       double y = 0.0;
@@ -861,7 +928,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
           a.logprobs[r] = (float)(-y * 0.69314718055994530942 - log((double)W / a.scale));
       }
     }
-    cl.sync();  // no block leaves while another may read its shared memory
+    cl.barrier_wait(std::move(here));
     return;
   }
 
@@ -988,6 +1055,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   const uint64_t mine_before = sh.pick_before, W = sh.pick_total;
   const uint32_t my_tie_base = sh.pick_ties;
   const double want = u * (double)W;
+  // nothing more is read from another block: one may leave when all are here
+  auto here = cl.barrier_arrive();
   // The block that has it: a thread per unit of that warp's part, in order.
   if (target_warp / WARPS == rank) {
     const int q0 = warp_begin(target_warp % WARPS), q1 = warp_begin(target_warp % WARPS + 1);
@@ -1074,7 +1143,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       }
     }
   }
-  cl.sync();  // no block leaves while another may read its shared memory
+  cl.barrier_wait(std::move(here));
 }
 
 template <typename T>
@@ -1154,7 +1223,11 @@ extern "C" int gq_sample(const void* logits, int dtype, int64_t rows, int64_t vo
   a.logprobs = logprobs;
   int log2v = 0;
   while ((1ll << log2v) < vocab) ++log2v;
-  a.scale = (double)(1ll << std::min(45, 62 - log2v));
+  const int bits = std::min(45, 62 - log2v);  // S: a term has S + 1 bits
+  a.scale = (double)(1ll << bits);
+  // 16 bits and at most 2^16 tokens a block for up to 2^19 tokens in 8 blocks (2^14
+  // each below 2^17); S = 42 for 2^20, and 15 bits of 2^17 tokens
+  a.limb = (bits + 3) / 3;
   cudaStream_t st = as_stream(stream);
   if (dtype == 0) return samp::run<float>(a, st);
   if (dtype == 1) return samp::run<__nv_bfloat16>(a, st);
