@@ -37,6 +37,17 @@ class PreparedLinear:
     granule: int            # columns that share one scale in the layout
     direct: bool            # positions are the columns in their own order
 
+    def __post_init__(self):
+        # the leading arguments of gq_linear, ready for every call
+        object.__setattr__(self, "_head", (
+            self.qweight.data_ptr(), self.params.data_ptr(), self.kmap.data_ptr(), self.m, self.n,
+            self.k, self.bits, self.granule, self.direct))
+        object.__setattr__(self, "_index", self.qweight.get_device())
+
+    def __reduce__(self):  # a copy has tensors, and so addresses, of its own
+        return PreparedLinear, (self.qweight, self.params, self.kmap, self.m, self.n, self.k,
+                                self.bits, self.granule, self.direct)
+
     @property
     def device(self) -> torch.device:
         return self.qweight.device
@@ -123,23 +134,21 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     exact bf16 terms) and rounded once.  numpy in -> numpy out.  ``out``, if
     given, is a contiguous tensor of the result's shape and type that does not
     share memory with ``x``."""
-    if A.is_host(x):
-        return A.like_input(packed_matmul(A.to_device(x), w), x)
-    dt = _DTYPES.get(x.dtype)
+    dt = _DTYPES.get(getattr(x, "dtype", None))
     if dt is None:
+        if A.is_host(x):
+            return A.like_input(packed_matmul(A.to_device(x), w), x)
         raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    n, m = w.n, w.m
+    n, m, dev = w.n, w.m, x.get_device()
     if x.dim() < 1 or x.shape[-1] != n:
         raise ValueError(f"x must be [..., {n}], got {tuple(x.shape)}")
-    dev = x.get_device()
-    if dev < 0 or dev != w.qweight.get_device():
+    if dev < 0 or dev != w._index:
         raise ValueError(f"x is on {x.device}, the weights on {w.qweight.device}")
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return packed_matmul(x, w, out)
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= n:
-        x2 = x
-    else:
+    x2 = x
+    if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) < n:
         x2 = x.reshape(-1, n).contiguous()
     tokens, ldx = x2.shape[0], x2.stride(0)
     if out is None:
@@ -158,9 +167,8 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
         nbytes = lib.gq_linear_workspace_size(tokens, w.k, dt)
         ws = A.workspace(nbytes)
         wp = ws.data_ptr()
-    status = lib.gq_linear(w.qweight.data_ptr(), w.params.data_ptr(), w.kmap.data_ptr(), m, n, w.k,
-                           w.bits, w.granule, w.direct, xp, dt, tokens, ldx, out.data_ptr(), m, wp,
-                           nbytes, A.raw_stream(dev))
+    status = lib.gq_linear(*w._head, xp, dt, tokens, ldx, out.data_ptr(), m, wp, nbytes,
+                           A.raw_stream(dev))
     if status:
         _lib.raise_status(status)
     return out

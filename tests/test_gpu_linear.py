@@ -13,6 +13,9 @@ rounding.  float32 terms below 2^-126 (the lowest bits of numbers under
 2^-110) are not among the inputs.
 """
 
+import copy
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -184,6 +187,18 @@ def test_of_a_gptq_result_and_module():
         amount = xt.double().abs() @ packing.dequantize(p).double().abs().T
         tol = (8 * 17 + 4 + 32 + 1) * 2.0 ** -23 * amount + 2.0 ** -24 * ref.abs()
         assert bool(((lin(xt).double() - ref).abs() <= tol).all())
+
+
+def test_copies_have_their_own_weights():
+    p, w = _packed(40, 256, 64, 4, False, 8, act_order=True)
+    lin = linear.QuantLinear(p)
+    x = _x((5, 256), torch.bfloat16, 1)
+    want = lin(x)
+    for other in (copy.deepcopy(lin), pickle.loads(pickle.dumps(lin))):
+        assert other.weights.qweight.data_ptr() != lin.weights.qweight.data_ptr()
+        lin.weights.qweight.zero_()
+        assert torch.equal(other(x), want)
+        lin = linear.QuantLinear(p)
 
 
 @pytest.mark.parametrize("t", [1, 8, 100, 260])
