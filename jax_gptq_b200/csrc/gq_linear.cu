@@ -35,6 +35,7 @@ namespace gq {
 namespace lin {
 
 constexpr int WARPS = 8;     // warps of a product CTA, which split K
+constexpr int MAX_PARTS = 8; // CTAs of a cluster, which split K again
 
 // ---------------------------------------------------------------- layout
 
@@ -207,24 +208,30 @@ struct Args {
   int tokens;
 };
 
-// One CTA: 16 rows, up to 8 NT columns; its warps take contiguous shares of K
-// and their sums are added in warp order.
+// One cluster: 16 rows, up to 8 NT columns; the warps of its CTAs take
+// contiguous shares of K and their sums are added in order.
 template <int WIDTH, typename T, int NT, int G>
-__global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2) few_kernel(Args a, bool dependent) {
+__global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2)
+    few_kernel(Args a, int split, bool dependent) {
   constexpr bool BF16 = !std::is_same<T, __half>::value;
   constexpr int SPLIT = std::is_same<T, float>::value ? 3 : 1;
   constexpr int TOK = 8 * NT / SPLIT;  // whole tokens per CTA
   constexpr int JG = G / 32;           // 32-position steps per granule
   constexpr int GPC = KC / G;          // granules per block
   constexpr int LPR = WIDTH / 4;       // 16-byte loads per lane, row and block
-  constexpr int DEPTH = 3;             // blocks in flight per warp
+  constexpr int DEPTH = 2;             // blocks in flight per warp; 3 and 4 spill or take a CTA
   __shared__ float red[WARPS][8 * NT][ROWS + 1];
+  __shared__ float sums[MAX_PARTS][8 * NT * ROWS];  // of the cluster's CTAs, in its first one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int64_t rb = blockIdx.x;
+  const int parts = 1 << split;                 // CTAs of the cluster
+  const int part = blockIdx.x & (parts - 1);    // this one's rank
+  const int64_t rb = blockIdx.x >> split;
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int tok0 = blockIdx.y * TOK;
   const int col0 = tok0 * SPLIT;
-  const int c0 = (int)((int64_t)a.nkc * warp / WARPS), c1 = (int)((int64_t)a.nkc * (warp + 1) / WARPS);
+  const int share = part * WARPS + warp;
+  const int c0 = (a.nkc * share / WARPS) >> split, c1 = (a.nkc * (share + 1) / WARPS) >> split;
   const uint4* qrow = a.qw + (rb * a.nkc) * (ROWS * 4 * LPR);
   const float2* prow = a.params + (rb * a.nkc) * (int64_t)(GPC * ROWS);
 
@@ -321,35 +328,66 @@ __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2) few_kernel(Args a
     for (int e = 0; e < 4; ++e)
       red[warp][8 * i + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[i][e];
   __syncthreads();
+  // every CTA is running: the first one's memory can be written to
+  if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  for (int i = threadIdx.x; i < TOK * ROWS; i += 32 * WARPS) {
+    const int r = i % ROWS, tk = i / ROWS;
+    float v = 0.f;
+#pragma unroll
+    for (int s = SPLIT - 1; s >= 0; --s) {  // the small terms first
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) sum += red[w][tk * SPLIT + s][r];
+      v += sum;
+    }
+    if (parts == 1) {
+      const int64_t row = rb * ROWS + r;
+      if (row < a.m && tok0 + tk < a.tokens)
+        store_out(static_cast<T*>(a.y) + (int64_t)(tok0 + tk) * a.ldy + row, v);
+    } else {
+      asm volatile(
+          "{\n.reg .b32 d;\nmapa.shared::cluster.u32 d, %0, 0;\n"
+          "st.shared::cluster.f32 [d], %1;\n}" ::"r"((uint32_t)__cvta_generic_to_shared(&sums[part][i])),
+          "f"(v)
+          : "memory");
+    }
+  }
+  if (parts == 1) return;
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (part) return;  // nothing reads the memory of the others
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   for (int i = threadIdx.x; i < TOK * ROWS; i += 32 * WARPS) {
     const int r = i % ROWS, tk = i / ROWS;
     const int64_t row = rb * ROWS + r;
     if (row >= a.m || tok0 + tk >= a.tokens) continue;
     float v = 0.f;
-#pragma unroll
-    for (int s = SPLIT - 1; s >= 0; --s) {  // the small terms first
-      float part = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) part += red[w][tk * SPLIT + s][r];
-      v += part;
-    }
+    for (int s = 0; s < parts; ++s) v += sums[s][i];
     store_out(static_cast<T*>(a.y) + (int64_t)(tok0 + tk) * a.ldy + row, v);
   }
 }
 
 template <typename... P, typename... A>
 cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                   bool dependent, A... args) {
+                   int cluster, bool dependent, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (dependent) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = (unsigned)cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = dependent ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -357,14 +395,20 @@ template <int WIDTH, typename T, int NT>
 int run_few(const Args& a, int granule, bool dependent, cudaStream_t st) {
   constexpr int SPLIT = std::is_same<T, float>::value ? 3 : 1;
   constexpr int TOK = 8 * NT / SPLIT;
-  const dim3 grid((unsigned)ceil_div(a.m, ROWS), (unsigned)ceil_div(a.tokens, TOK));
+  const int64_t rbs = ceil_div(a.m, ROWS), groups = ceil_div(a.tokens, TOK);
+  // K is split over a cluster while there are fewer CTAs than SMs and every warp
+  // keeps a block: 1 token of 1024 x 8192 3.5 us by clusters of 4, 5.5 by single
+  // CTAs; of 4096 x 4096 (256 row blocks) 6.8 by pairs, 4.3 without.
+  int split = 0;
+  while ((1 << split) < MAX_PARTS && (rbs * groups << split) < 148 && a.nkc >= 2 * WARPS << split) ++split;
+  const dim3 grid((unsigned)(rbs << split), (unsigned)groups);
   cudaError_t e;
   if (granule == 128)
-    e = launch(few_kernel<WIDTH, T, NT, 128>, grid, dim3(32 * WARPS), 0, st, dependent, a, dependent);
+    e = launch(few_kernel<WIDTH, T, NT, 128>, grid, dim3(32 * WARPS), 0, st, 1 << split, dependent, a, split, dependent);
   else if (granule == 64)
-    e = launch(few_kernel<WIDTH, T, NT, 64>, grid, dim3(32 * WARPS), 0, st, dependent, a, dependent);
+    e = launch(few_kernel<WIDTH, T, NT, 64>, grid, dim3(32 * WARPS), 0, st, 1 << split, dependent, a, split, dependent);
   else
-    e = launch(few_kernel<WIDTH, T, NT, 32>, grid, dim3(32 * WARPS), 0, st, dependent, a, dependent);
+    e = launch(few_kernel<WIDTH, T, NT, 32>, grid, dim3(32 * WARPS), 0, st, 1 << split, dependent, a, split, dependent);
   if (e != cudaSuccess) return fail(GQ_ECUDA, "gq_linear: %s", cudaGetErrorString(e));
   return check_launch("gq_linear few-token product");
 }

@@ -53,6 +53,14 @@ __device__ __forceinline__ uint32_t offset_operand(float o) {
   else return pack2<false>(1024.f + o, 1024.f + o);
 }
 
+// (x & mask) | bits as the one instruction it is: left to the compiler it took
+// two, and a one-token product of 28672 x 8192 36.2 us in place of 33.8.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(mask), "r"(bits));
+  return d;
+}
+
 // The four pairs (code - offset) of 8 positions.  4-bit fields are moved into
 // the mantissa of 16.0, where they count in ones: bits 3-6 of a bf16, bits 6-9
 // of an fp16; 8-bit fields into the mantissa of 2^23 (float) or 1024 (fp16).
@@ -65,9 +73,9 @@ __device__ __forceinline__ void decode8(const uint32_t* w, uint32_t off, uint32_
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       if constexpr (BF16)
-        v[p] = (__funnelshift_r(x, x, 4 * p) & 0x00780078u) | 0x41804180u;
+        v[p] = and_or(__funnelshift_r(x, x, 4 * p), 0x00780078u, 0x41804180u);
       else
-        v[p] = (__funnelshift_r(x, x, (4 * p + 29) & 31) & 0x03c003c0u) | 0x4c004c00u;
+        v[p] = and_or(__funnelshift_r(x, x, (4 * p + 29) & 31), 0x03c003c0u, 0x4c004c00u);
     }
 #pragma unroll
     for (int p = 0; p < 4; ++p) v[p] = sub2<BF16>(v[p], off);
