@@ -16,7 +16,7 @@
 // sums of whole numbers do not depend on the order of additions, so the shared
 // memory atomics and the split over threads and blocks never change a result,
 // and a term's rounding (2^-46 of the largest) is far below what a float32
-// uniform resolves.  Terms below 2^-(S+1) are zero: they can not be drawn.
+// uniform resolves.  Terms below 2^-(S+1) are rounded to zero: they can not be drawn.
 //
 // Split.  A cluster of up to 8 blocks takes a row, each a contiguous part, each
 // warp a contiguous part of that, kept in shared memory (up to 131072 tokens in
@@ -111,44 +111,62 @@ __device__ __forceinline__ float from_ordered(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
 
-// 2^-y for 0 <= y < 1000, within 2^-47 of it: y is split at the nearest whole
-// number and 2^f, |f| <= 1/2, is the Taylor series of exp(f ln 2) to the 11th power
-// (remainder below 7e-15).  N at a time, step by step: one alone is a chain of 18
-// dependent float64 operations, and four warps a scheduler do not hide that.
+// 2^(-j/32), the nearest doubles
+constexpr int ROOTS = 32;
+__device__ const uint64_t root_bits[ROOTS] = {
+    0x3ff0000000000000ull, 0x3fef50765b6e4540ull, 0x3feea4afa2a490daull, 0x3fedfc97337b9b5full,
+    0x3fed5818dcfba487ull, 0x3fecb720dcef9069ull, 0x3fec199bdd85529cull, 0x3feb7f76f2fb5e47ull,
+    0x3feae89f995ad3adull, 0x3fea5503b23e255dull, 0x3fe9c49182a3f090ull, 0x3fe93737b0cdc5e5ull,
+    0x3fe8ace5422aa0dbull, 0x3fe82589994cce13ull, 0x3fe7a11473eb0187ull, 0x3fe71f75e8ec5f74ull,
+    0x3fe6a09e667f3bcdull, 0x3fe6247eb03a5585ull, 0x3fe5ab07dd485429ull, 0x3fe5342b569d4f82ull,
+    0x3fe4bfdad5362a27ull, 0x3fe44e086061892dull, 0x3fe3dea64c123422ull, 0x3fe371a7373aa9cbull,
+    0x3fe306fe0a31b715ull, 0x3fe29e9df51fdee1ull, 0x3fe2387a6e756238ull, 0x3fe1d4873168b9aaull,
+    0x3fe172b83c7d517bull, 0x3fe11301d0125b51ull, 0x3fe0b5586cf9890full, 0x3fe059b0d3158574ull};
+struct Roots {  // in shared memory, high and low words: one a bank each
+  uint32_t hi[ROOTS], lo[ROOTS];
+};
+
+// 2^-y for 0 <= y < 1000, within 2^-47 of it: y is split at the nearest k/32,
+// 2^-(k/32) is a table's entry with an exponent, and 2^-f, |f| <= 1/64, is the Taylor
+// series to the 5th power (remainder below 2^-48).  N at a time, step by step: one
+// alone is a chain of dependent float64 operations, and four warps a scheduler do not
+// hide that.
 template <int N>
-__device__ __forceinline__ void exp2_neg(const double (&y)[N], double (&out)[N]) {
+__device__ __forceinline__ void exp2_neg(const Roots& roots, const double (&y)[N], double (&out)[N]) {
   constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the whole part
-  constexpr double c[12] = {1.0, 1.0, 0.5, 1.6666666666666666e-01, 4.1666666666666664e-02,
-                            8.333333333333333e-03, 1.388888888888889e-03, 1.984126984126984e-04,
-                            2.48015873015873e-05, 2.755731922398589e-06, 2.755731922398589e-07,
-                            2.505210838544172e-08};  // 1 / n!
+  constexpr double c[6] = {1.0, -0.6931471805599453, 0.24022650695910072, -0.05550410866482158,
+                           0.009618129107628477, -0.0013333558146428443};  // (-ln 2)^n / n!
   double x[N];
-  int n[N];
+  int k[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const double s = magic - y[i];
-    n[i] = __double2loint(s);
-    x[i] = ((magic - s) - y[i]) * 0.69314718055994530942;
-    out[i] = c[11];
+    const double s = fma(y[i], (double)ROOTS, magic);
+    k[i] = __double2loint(s);
+    x[i] = fma(s - magic, -1.0 / ROOTS, y[i]);
+    out[i] = c[5];
   }
 #pragma unroll
-  for (int k = 10; k >= 0; --k)
+  for (int n = 4; n >= 0; --n)
 #pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = fma(out[i], x[i], c[k]);
+    for (int i = 0; i < N; ++i) out[i] = fma(out[i], x[i], c[n]);
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    out[i] = __hiloint2double(__double2hiint(out[i]) + (n[i] << 20), __double2loint(out[i]));
+  for (int i = 0; i < N; ++i) {
+    const int j = k[i] & (ROOTS - 1);
+    out[i] *= __hiloint2double((int)roots.hi[j] - ((k[i] << 15) & (int)0xfff00000), (int)roots.lo[j]);
+  }
 }
 
 struct Row {
   double mx, c;  // the maximum, log2(e) / temperature
-  double limit;  // terms with log2 e below -limit are zero
+  double limit;  // terms with log2 e below -limit are zero: S + 2, where rounding makes them so too
   double scale;
+  float top, low;  // the maximum; a logit whose term is zero
+  bool plain;      // `low` is so, and (mx - l) c below 1000 for all l from there on
+  const Roots* roots;
   // distance below the maximum in powers of two; false where the term is zero
   // (y is then any number)
   __device__ __forceinline__ bool distance(float l, double& y) const {
-    const double v = (double)l;
-    y = v == mx ? 0.0 : (mx - v) * c;
+    y = l == top ? 0.0 : (mx - (double)l) * c;
     return y < limit;  // false for NaN
   }
   // the terms as whole numbers, 0 where !have
@@ -156,12 +174,25 @@ struct Row {
   __device__ __forceinline__ void fixed(const double (&y)[N], const bool (&have)[N],
                                         uint64_t (&f)[N]) const {
     double e[N];
-    exp2_neg(y, e);
+    exp2_neg(*roots, y, e);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const double t = fma(e[i], scale, 4503599627370496.0);  // + 2^52: whole number in the low bits
       f[i] = have[i] ? (uint64_t)__double_as_longlong(t) & 0xfffffffffffffull : 0;
     }
+  }
+  // the sum of four logits' terms (plain rows): those below `low` and NaN are raised to
+  // it, and only the sum is freed of the four exponents of 2^52
+  __device__ __forceinline__ uint64_t sum4(const float* l) const {
+    double y[4], e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = (mx - (double)fmaxf(l[i], low)) * c;
+    exp2_neg(*roots, y, e);
+    uint64_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      sum += (uint64_t)__double_as_longlong(fma(e[i], scale, 4503599627370496.0));
+    return sum - 4 * 0x4330000000000000ull;
   }
   __device__ __forceinline__ uint64_t fixed(float l) const {
     double y[1];
@@ -219,6 +250,7 @@ struct Border {
 };
 
 struct Shared {
+  Roots roots;
   uint32_t count[BINS];                // histogram over log2 e: tokens
   uint32_t mass[3][BINS];              // and sums, by limbs of a.limb bits
   union {
@@ -272,9 +304,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   // f(values, index of the first) for this lane's tokens, a unit at a time, NaN
   // where there is none
   auto each_unit = [&](auto&& f) {
+    if (w0 + lane >= w1) return;
+    uint4 next = unit(w0 + lane);  // one ahead: a row that is not staged comes from L2
     for (int q = w0 + lane; q < w1; q += 32) {
       float x[VEC];
-      un.values(unit(q), x);
+      un.values(next, x);
+      if (q + 32 < w1) next = unit(q + 32);
       f(x, q * VEC - un.shift);
     }
   };
@@ -292,6 +327,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   const double p = row_value(a.top_p, r);
   const double mp = row_value(a.min_p, r);
   const double u = row_value(a.u, r);
+
+  const uint64_t root = tid < ROOTS ? root_bits[tid] : 0;
 
   // ---- 1. the maximum (and for temperature 0 its first index)
   float mx = -INFINITY;
@@ -329,6 +366,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     sh.amax[warp] = arg;
   }
   sh.count[tid] = sh.mass[0][tid] = sh.mass[1][tid] = sh.mass[2][tid] = 0;
+  if (tid < ROOTS) {
+    sh.roots.hi[tid] = (uint32_t)(root >> 32);
+    sh.roots.lo[tid] = (uint32_t)root;
+  }
   if (tid == 0) {
     sh.list_n = 0;
     sh.hit = sh.last = -1;
@@ -376,9 +417,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   }
   Row rw;
   rw.mx = (double)mx;
+  rw.top = mx;
+  rw.roots = &sh.roots;
   rw.c = fmin(1.4426950408889634 / temp, 1e300);
   rw.scale = a.scale;
-  rw.limit = (double)(((__double2hiint(a.scale) >> 20) & 0x7ff) - 1023) + 1.0;  // S + 1
+  rw.limit = (double)(((__double2hiint(a.scale) >> 20) & 0x7ff) - 1023) + 2.0;  // S + 2
+  rw.low = __double2float_rd(rw.mx - 60.0 / rw.c);
+  const double low_y = (rw.mx - (double)rw.low) * rw.c;  // 0 where the largest is huge, NaN where infinite
+  rw.plain = rw.low > -INFINITY && low_y > 59.0 && low_y < 1000.0;
   const float cf = (float)fmin(rw.c, 3e38);
   // bin of a token; the last bin holds only terms that are zero (46.45 powers of
   // two below the largest and further), and whatever is no token at all
@@ -405,16 +451,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     each_unit([&](const float (&x)[VEC], int) {
 #pragma unroll
       for (int h = 0; h < VEC; h += 4) {
-        double y[4];
-        bool have[4];
-        uint64_t f[4];
+        if (rw.plain) {
+          sum += rw.sum4(x + h);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          have[e] = rw.distance(x[h + e], y[e]);
-          y[e] = have[e] ? y[e] : 0.0;
+          for (int e = 0; e < 4; ++e) sum += rw.fixed(x[h + e]);
         }
-        rw.fixed(y, have, f);
-        sum += f[0] + f[1] + f[2] + f[3];
       }
     });
     sum = warp_sum64(sum);
@@ -1148,11 +1190,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
 
 template <typename T>
 int run(const Args& a, cudaStream_t st) {
-  // Blocks of a row: as many as leave each at least 2048 tokens, while that leaves
-  // SMs idle; at least one for every 16384 tokens, so that a part fits shared memory.
   int cluster = 1;
-  while (cluster < MAX_CL && a.vocab > 16384 * cluster) cluster *= 2;
-  while (cluster < MAX_CL && a.rows * cluster * 2 <= sm_count() && a.vocab >= 2048 * 2 * cluster)
+  const auto rows_at_once = [&] { return std::min<int64_t>(a.rows, 2 * sm_count() / cluster); };
+  while (cluster < MAX_CL && a.vocab >= 4096 * cluster &&
+         (a.rows * cluster * 2 <= sm_count() ||
+          (a.vocab >= 12288 * cluster && a.rows * cluster <= sm_count()) ||
+          rows_at_once() * a.vocab * (int64_t)sizeof(T) > (96 << 20)))
     cluster *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * cluster));
