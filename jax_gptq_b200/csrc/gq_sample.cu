@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     for (int q = w0 + lane; q < w1; q += 32) {
       float x[VEC];
       un.values(next, x);
-      if (q + 32 < w1) next = unit(q + 32);
+      next = unit(min(q + 32, w1 - 1));
       f(x, q * VEC - un.shift);
     }
   };
@@ -344,12 +344,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       if (STAGED) stage[q + 32 * i - b0] = raw[i];
       float x[VEC];
       un.values(raw[i], x);
+      if (temp > 0.0) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (x[e] > mx) {  // indices grow along a lane's walk: the first one stays
-          mx = x[e];
-          arg = (uint32_t)((q + 32 * i) * VEC - un.shift + e);
-        }
+        for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, x[e]);  // (not NaN)
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (x[e] > mx) {  // indices grow along a lane's walk: the first one stays
+            mx = x[e];
+            arg = (uint32_t)((q + 32 * i) * VEC - un.shift + e);
+          }
+      }
     }
   }
 #pragma unroll
