@@ -19,8 +19,8 @@
 // uniform resolves.  Terms below 2^-(S+1) are rounded to zero: they can not be drawn.
 //
 // Split.  A cluster of up to 8 blocks takes a row, each a contiguous part, each
-// warp a contiguous part of that, kept in shared memory (up to 131072 tokens in
-// float32; longer rows are read again from L1 and L2).  Passes over the row:
+// warp a contiguous part of that; parts of up to 64 KB are kept in shared memory,
+// larger ones are read again from L2.  Passes over the row:
 //   1. the maximum;
 //   2. with top-k or top-p the number of tokens in 512 bins of log2 e (found in
 //      float32: any function that keeps the order will do); without top-k each
@@ -1195,10 +1195,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
 
 template <typename T>
 int run(const Args& a, cudaStream_t st) {
+  // Blocks of a row: as many as leave each at least 2048 tokens while the row's
+  // blocks do not fill half the slots (two to an SM); beyond that, as many as fill
+  // them once, with at least 6144 tokens each: larger clusters spend their time in
+  // the exchanges between blocks.  More only where the rows that run at once would
+  // not stay in L2 for the second pass.  256 x 128256 bf16, top-k 50 and top-p 0.95:
+  // 126 us by clusters of 8, 85 by 4, 75 by 2, 65 by 1; float32: 138, 110, 93, 118;
+  // 48 rows bf16: 30, 23, 29, 29.  (And no block more than 120000: see a.limb.)
   int cluster = 1;
   const auto rows_at_once = [&] { return std::min<int64_t>(a.rows, 2 * sm_count() / cluster); };
   while (cluster < MAX_CL && a.vocab >= 4096 * cluster &&
-         (a.rows * cluster * 2 <= sm_count() ||
+         (a.vocab > 120000 * cluster || a.rows * cluster * 2 <= sm_count() ||
           (a.vocab >= 12288 * cluster && a.rows * cluster <= sm_count()) ||
           rows_at_once() * a.vocab * (int64_t)sizeof(T) > (96 << 20)))
     cluster *= 2;
@@ -1273,9 +1280,10 @@ extern "C" int gq_sample(const void* logits, int dtype, int64_t rows, int64_t vo
   while ((1ll << log2v) < vocab) ++log2v;
   const int bits = std::min(45, 62 - log2v);  // S: a term has S + 1 bits
   a.scale = (double)(1ll << bits);
-  // 16 bits and at most 2^16 tokens a block for up to 2^19 tokens in 8 blocks (2^14
-  // each below 2^17); S = 42 for 2^20, and 15 bits of 2^17 tokens
-  a.limb = (bits + 3) / 3;
+  // The low limbs are below 2^limb, the high one at most 2^(S - 2 limb): 15 bits for S
+  // from 43 to 45, at most 120000 tokens a block (run() sees to that); 14 for S = 42
+  // (2^20 tokens in 8 blocks).  Either way a block's sum of one stays below 2^32.
+  a.limb = (bits + 2) / 3;
   cudaStream_t st = as_stream(stream);
   if (dtype == 0) return samp::run<float>(a, st);
   if (dtype == 1) return samp::run<__nv_bfloat16>(a, st);

@@ -216,6 +216,18 @@ def test_logprob_is_what_the_evaluation_scores():
     assert abs(nll + float(got.logprobs.double().sum())) <= 1e-5 * abs(nll)
 
 
+@pytest.mark.parametrize("rows,vocab", [(150, 110000), (2, 1 << 20)])
+def test_flat_rows(rows, vocab):
+    """Nearly all of a block's tokens in one cell: its sums have to have room for
+    that many terms, however many tokens the block has."""
+    z = (-(64 + torch.arange(rows, device="cuda")) / 256)[:, None].repeat(1, vocab)
+    z[:, torch.arange(vocab, device="cuda") % 11 > 8] -= 1 / 256  # the border is among these
+    z = z.bfloat16()
+    z[:, 3] = 0
+    u = torch.rand((rows,), generator=torch.Generator(device="cuda").manual_seed(rows), device="cuda")
+    _check(z, u, top_p=0.95)
+
+
 def test_streams_and_graphs():
     z, u = _logits(8, 32000, torch.bfloat16, 13)
     kw = dict(temperature=0.8, top_k=50, top_p=0.9)
