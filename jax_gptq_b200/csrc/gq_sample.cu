@@ -31,11 +31,13 @@
 //      are collected and sorted by every block, and the borders read off their
 //      running sum; up to 256 kept ones are drawn from right there.
 //      Otherwise (flat distributions) top-k's border bin alone is sorted; for top-p
-//      the counts also tell from which bin on the border can lie (a bin's sum is at
-//      most its count times its largest e), one pass adds up what lies before and
-//      512 cells between the two, and the border's cell is sorted.  More than 2048
-//      tokens in one (runs of equal logits) are resolved by radix passes over the
-//      ordered bits;
+//      the bins' sums are estimated, and one pass adds up what lies before the place
+//      where the border should be and collects the tokens around it.  Where that
+//      misses, the counts also tell from which bin on the border can lie (a bin's sum
+//      is at most its count times its largest e), one pass adds up what lies before
+//      and 512 cells between the two, and the border's cell is sorted.  More than
+//      2048 tokens in one (runs of equal logits) are resolved by radix passes over
+//      the ordered bits;
 //   4. with filters each warp's sum of the kept e and its number of tokens equal
 //      to the border;
 //   5. the block that holds u W finds the token in the part of one warp.
@@ -283,6 +285,55 @@ struct Shared {
   int hit, last;
   double hit_y, last_y;
 };
+
+// Sorts E keys a thread, the largest first, by a bitonic network: keys E t .. E t + E - 1
+// in thread t's registers, partners in other lanes by shuffles, in other warps through
+// shared memory (10 of 66 steps of 2048 keys; 812 keys took 19000 cycles with all
+// steps there, 9300 so).
+template <int E>
+__device__ __forceinline__ void sort_keys(unsigned long long* keys) {
+  const int tid = threadIdx.x;
+  struct alignas(16) Pack { unsigned long long k[E]; } v;
+  __syncthreads();
+  v = reinterpret_cast<const Pack*>(keys)[tid];
+  auto exchange = [](unsigned long long mine, unsigned long long other, bool larger) {
+    return (mine > other) == larger ? mine : other;
+  };
+  for (int k = 2; k <= E * THREADS; k *= 2) {
+    for (int j = k / 2; j >= E; j /= 2) {
+      const bool larger = ((E * tid & j) == 0) == ((E * tid & k) == 0);
+      const int apart = j / E;  // threads
+      Pack o;
+      if (apart < 32) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) o.k[i] = __shfl_xor_sync(0xffffffffu, v.k[i], apart);
+      } else {
+        __syncthreads();
+        reinterpret_cast<Pack*>(keys)[tid] = v;
+        __syncthreads();
+        o = reinterpret_cast<const Pack*>(keys)[tid ^ apart];
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) v.k[i] = exchange(v.k[i], o.k[i], larger);
+    }
+#pragma unroll
+    for (int j = E / 2; j > 0; j /= 2) {  // inside the thread
+      if (j >= k) continue;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if ((i & j) == 0) {
+          const bool larger = ((E * tid + i) & k) == 0;
+          const unsigned long long x = v.k[i], y = v.k[i + j];
+          const bool keep = (x > y) == larger;
+          v.k[i] = keep ? x : y;
+          v.k[i + j] = keep ? y : x;
+        }
+    }
+  }
+  __syncthreads();
+  reinterpret_cast<Pack*>(keys)[tid] = v;
+  __syncthreads();
+}
 
 // STAGED: the block's part of the row is kept in shared memory
 template <typename T, bool STAGED>
@@ -539,16 +590,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   // is earlier.  The number of them over the whole row; if that is at most LIST they
   // are in the blocks' `list`s, block c's ending at `upto` of lane c.
   uint32_t upto = 0;
-  auto collect = [&](auto&& pred) {
-    __syncthreads();
-    if (tid == 0) sh.list_n = 0;
-    __syncthreads();
-    each_token([&](float x, int i) {
-      if (!pred(x)) return;
-      const uint32_t at = atomicAdd(&sh.list_n, 1u);
-      if (at < LIST) sh.list[at] = (unsigned long long)ordered(x) << 32 | ~(uint32_t)i;
-    });
-    cl.sync();
+  auto listed = [&] {  // once every block's list is complete
     upto = lane < CL ? peer(lane)->list_n : 0;
 #pragma unroll
     for (int o = 1; o < MAX_CL; o <<= 1) {
@@ -559,11 +601,28 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     if (n > LIST) cl.sync();  // the lists are not read further and may be begun anew
     return n;
   };
+  auto list_token = [&](float x, int i) {
+    const uint32_t at = atomicAdd(&sh.list_n, 1u);
+    if (at < LIST) sh.list[at] = (unsigned long long)ordered(x) << 32 | ~(uint32_t)i;
+  };
+  auto begin_list = [&] {
+    __syncthreads();
+    if (tid == 0) sh.list_n = 0;
+    __syncthreads();
+  };
+  auto collect = [&](auto&& pred) {
+    begin_list();
+    each_token([&](float x, int i) {
+      if (pred(x)) list_token(x, i);
+    });
+    cl.sync();
+    return listed();
+  };
   // The n <= LIST collected tokens of all blocks in `keys`, the earliest first.
   auto sorted = [&](uint32_t n) {
-    uint32_t size = 64;
-    while (size < n) size *= 2;
-    for (uint32_t i = tid; i < ((size + 31) & ~31u); i += THREADS) {
+    // (only ranked ones need no full array)
+    const uint32_t size = n <= RANKED ? (n + 31) & ~31u : n <= 2 * THREADS ? 2 * THREADS : LIST;
+    for (uint32_t i = tid; i < size; i += THREADS) {
       unsigned long long key = 0;  // below every token
       uint32_t c = 0, from = 0;
 #pragma unroll
@@ -575,7 +634,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
         }
       }
       if (i < n) key = peer(c)->list[i - from];
-      if (i < size) sh.keys[i] = key;
+      sh.keys[i] = key;
     }
     if (n <= RANKED) {
       __syncthreads();
@@ -593,23 +652,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       __syncthreads();
       return;
     }
-    // bitonic network; pairs up to 32 apart stay inside a warp's 64 keys
-    uint32_t last = 64;
-    for (uint32_t k2 = 2; k2 <= size; k2 *= 2)
-      for (uint32_t j = k2 / 2; j > 0; j /= 2) {
-        if (j > 32 || last > 32) __syncthreads();
-        else __syncwarp();
-        last = j;
-        for (uint32_t t = tid; t < size / 2; t += THREADS) {
-          const uint32_t i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
-          const unsigned long long x = sh.keys[i], y = sh.keys[i + j];
-          if (((i & k2) == 0) == (x < y)) {
-            sh.keys[i] = y;
-            sh.keys[i + j] = x;
-          }
-        }
-      }
-    __syncthreads();
+    if (n <= 2 * THREADS) sort_keys<2>(sh.keys);
+    else sort_keys<4>(sh.keys);
   };
   auto sorted_value = [&](uint32_t i) { return from_ordered((uint32_t)(sh.keys[i] >> 32)); };
   // The terms of the first n sorted tokens, EACH a thread, with their running sum;
@@ -849,83 +893,137 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
             target = fmax(p, 0.0) * (double)(add_up(mine) + border.ties * each);
           }
           cl.sync();  // wmass is read and may be written again
-          // the first bin by whose end the sum can have reached the target: a bin's sum
-          // is at most its count times its largest e
-          const unsigned long long most = (unsigned long long)(
-              hc * (double)exp2f(-((float)tid - 0.01f) / 11.f) * 1.0001 * rw.scale) + hc;
-          unsigned long long pm;
-          uint32_t pn, tn;
-          scan(most, 0, pm, pn, tm, tn);
-          const int low =
-              max(tell((double)pm < target && !((double)(pm + most) < target) ? tid : -1, 0, 0, 0, 0), 0);
-          // one pass: the sum of what lies before bin `low`, and of each of 512 cells
-          // between there and bin `limit`
-          const float split = (float)max(1, BINS / max(1, limit + 1 - min(low, limit)));
-          const float first_depth = (float)min(low, limit), end_depth = (float)(limit + 1);
-          auto cell = [&](float x) {  // -1 before, BINS behind
-            const float d = depth(x);
-            if (!(d < end_depth) || (cut_k && ordered(x) <= above)) return BINS;
-            return d < first_depth ? -1 : min(BINS - 1, (int)((d - first_depth) * split));
-          };
-          uint64_t before = 0;
-          each_unit([&](const float (&x)[VEC], int) {
+          // Where the border is likely to be: the bins' sums estimated halfway between
+          // their bounds, a bin's tokens spread evenly; up and down from there 0.25 % of the
+          // target, but at least 200 tokens and at most 800.  One pass adds up what lies
+          // before and collects what lies there: a flat row of 128256 bf16 tokens takes 32
+          // to 40 us, by the cells below 45 to 62.  Not found there, it is looked for so.
+          bool found = false;
+          if (!cut_k && rw.plain) {
+            const unsigned long long most = (unsigned long long)(
+                hc * (double)exp2f(-((float)tid - 0.01f) / 11.f) * 1.0001 * rw.scale);
+            const unsigned long long half = least / 2 + most / 2;
+            unsigned long long pe, te;
+            uint32_t pn, tn;
+            scan(half, 0, pe, pn, te, tn);
+            const double ratio = (double)z / (double)te;
+            const double b = (double)pe * ratio, e = (double)(pe + half) * ratio;
+            auto place = [&](double t, float otherwise) {  // depth at which the sum should be t
+              const bool mine = b < t && !(e < t);
+              const int bin = tell(mine ? tid : -1, 0, mine ? (unsigned long long)__double_as_longlong((t - b) / (e - b)) : 0, 0, 0);
+              return bin < 0 ? otherwise : (float)bin + (float)__longlong_as_double((long long)sh.found_mass);
+            };
+            const double about = exp2f(place(target, (float)(BINS - 1)) / -11.f) * rw.scale;  // a term there
+            const double off = fmin(fmax(0.0025 * target, 200.0 * about), 800.0 * about);
+            const float from = place(target - off, 0.f), to = place(target + off, (float)(BINS - 1));
+            begin_list();
+            uint64_t before = 0;
+            each_unit([&](const float (&x)[VEC], int i) {
 #pragma unroll
-            for (int h = 0; h < VEC; h += 4) {
-              double y[4];
-              bool have[4];
-              int c[4];
-              uint64_t f[4];
+              for (int h = 0; h < VEC; h += 4) {
+                float v[4];
+                bool any = false;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                c[e] = cell(x[h + e]);
-                have[e] = c[e] < BINS && rw.distance(x[h + e], y[e]);
-                y[e] = have[e] ? y[e] : 0.0;
-              }
-              if (!(have[0] || have[1] || have[2] || have[3])) continue;
-              rw.fixed(y, have, f);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (!have[e]) continue;
-                if (c[e] < 0) {
-                  before += f[e];
-                } else {  // (64-bit additions here took 5 times as long)
-                  const uint32_t mask = (1u << a.limb) - 1u;
-                  atomicAdd(&sh.mass[0][c[e]], (uint32_t)f[e] & mask);
-                  atomicAdd(&sh.mass[1][c[e]], (uint32_t)(f[e] >> a.limb) & mask);
-                  atomicAdd(&sh.mass[2][c[e]], (uint32_t)(f[e] >> 2 * a.limb));
+                for (int e = 0; e < 4; ++e) {
+                  const float d = depth(x[h + e]);
+                  v[e] = d < from ? x[h + e] : rw.low;
+                  any |= d < from;
+                  if (d >= from && d < to) list_token(x[h + e], i + h + e);
                 }
+                if (any) before += rw.sum4(v);
               }
-            }
-          });
-          const unsigned long long base = add_up(before);
-          unsigned long long hm = 0;
-#pragma unroll
-          for (int c = 0; c < MAX_CL; ++c)
-            if (c < CL) {
-              const Shared* o = peer(c);
-              hm += o->mass[0][tid] + ((unsigned long long)o->mass[1][tid] << a.limb) +
-                    ((unsigned long long)o->mass[2][tid] << 2 * a.limb);
-            }
-          scan(hm, 0, pm, pn, tm, tn);
-          pm += base;
-          // the last cell that begins before the target
-          const int fc = tell((double)pm < target && !((double)(pm + hm) < target) ? tid : -1, 0, pm, 0, 0);
-          const unsigned long long msum = sh.found_mass;
-          if (fc >= 0) {
-            auto member = [&](float x) { return cell(x) == fc; };
-            n = collect(member);
+            });
+            const unsigned long long base = add_up(before);
+            n = listed();
             if (n <= LIST) {
               sorted(n);
               uint64_t f[EACH];
-              unsigned long long total;
+              unsigned long long pm, total;
               running(n, f, pm, total);
-              border_at(last_before(n, f, pm + msum, target), border);
-            } else {
-              radix(member, true, 0, msum, target, border);
+              found = (double)base < target && !((double)(base + total) < target);
+              if (found) border_at(last_before(n, f, pm + base, target), border);
+              cl.sync();  // the lists are read, as is wmass
             }
-          } else {
-            if (cut_k) border.ties = staying(border.ties, each, base + tm, target);  // among equal ones
-            cl.sync();  // as above
+          }
+          if (!found) {
+            // the first bin by whose end the sum can have reached the target: a bin's sum
+            // is at most its count times its largest e
+            const unsigned long long most = (unsigned long long)(
+                hc * (double)exp2f(-((float)tid - 0.01f) / 11.f) * 1.0001 * rw.scale) + hc;
+            unsigned long long pm;
+            uint32_t pn, tn;
+            scan(most, 0, pm, pn, tm, tn);
+            const int low =
+                max(tell((double)pm < target && !((double)(pm + most) < target) ? tid : -1, 0, 0, 0, 0), 0);
+            // one pass: the sum of what lies before bin `low`, and of each of 512 cells
+            // between there and bin `limit`
+            const float split = (float)max(1, BINS / max(1, limit + 1 - min(low, limit)));
+            const float first_depth = (float)min(low, limit), end_depth = (float)(limit + 1);
+            auto cell = [&](float x) {  // -1 before, BINS behind
+              const float d = depth(x);
+              if (!(d < end_depth) || (cut_k && ordered(x) <= above)) return BINS;
+              return d < first_depth ? -1 : min(BINS - 1, (int)((d - first_depth) * split));
+            };
+            uint64_t before = 0;
+            each_unit([&](const float (&x)[VEC], int) {
+#pragma unroll
+              for (int h = 0; h < VEC; h += 4) {
+                double y[4];
+                bool have[4];
+                int c[4];
+                uint64_t f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  c[e] = cell(x[h + e]);
+                  have[e] = c[e] < BINS && rw.distance(x[h + e], y[e]);
+                  y[e] = have[e] ? y[e] : 0.0;
+                }
+                if (!(have[0] || have[1] || have[2] || have[3])) continue;
+                rw.fixed(y, have, f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if (!have[e]) continue;
+                  if (c[e] < 0) {
+                    before += f[e];
+                  } else {  // (64-bit additions here took 5 times as long)
+                    const uint32_t mask = (1u << a.limb) - 1u;
+                    atomicAdd(&sh.mass[0][c[e]], (uint32_t)f[e] & mask);
+                    atomicAdd(&sh.mass[1][c[e]], (uint32_t)(f[e] >> a.limb) & mask);
+                    atomicAdd(&sh.mass[2][c[e]], (uint32_t)(f[e] >> 2 * a.limb));
+                  }
+                }
+              }
+            });
+            const unsigned long long base = add_up(before);
+            unsigned long long hm = 0;
+#pragma unroll
+            for (int c = 0; c < MAX_CL; ++c)
+              if (c < CL) {
+                const Shared* o = peer(c);
+                hm += o->mass[0][tid] + ((unsigned long long)o->mass[1][tid] << a.limb) +
+                      ((unsigned long long)o->mass[2][tid] << 2 * a.limb);
+              }
+            scan(hm, 0, pm, pn, tm, tn);
+            pm += base;
+            // the last cell that begins before the target
+            const int fc = tell((double)pm < target && !((double)(pm + hm) < target) ? tid : -1, 0, pm, 0, 0);
+            const unsigned long long msum = sh.found_mass;
+            if (fc >= 0) {
+              auto member = [&](float x) { return cell(x) == fc; };
+              n = collect(member);
+              if (n <= LIST) {
+                sorted(n);
+                uint64_t f[EACH];
+                unsigned long long total;
+                running(n, f, pm, total);
+                border_at(last_before(n, f, pm + msum, target), border);
+              } else {
+                radix(member, true, 0, msum, target, border);
+              }
+            } else {
+              if (cut_k) border.ties = staying(border.ties, each, base + tm, target);  // among equal ones
+              cl.sync();  // as above
+            }
           }
         }
       }
@@ -994,6 +1092,20 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) any |= x[e] >= border_value;
       if (!any) return;
+      if (rw.plain && !by_min) {
+#pragma unroll
+        for (int h = 0; h < VEC; h += 4) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool tie = x[h + e] == border_value && border.key != 0;
+            ties += tie;
+            v[e] = x[h + e] >= border_value && !tie ? x[h + e] : rw.low;
+          }
+          sum += rw.sum4(v);
+        }
+        return;
+      }
 #pragma unroll
       for (int h = 0; h < VEC; h += 4) {
         double y[4];
@@ -1201,11 +1313,11 @@ int run(const Args& a, cudaStream_t st) {
   // the exchanges between blocks.  More only where the rows that run at once would
   // not stay in L2 for the second pass.  256 x 128256 bf16, top-k 50 and top-p 0.95:
   // 126 us by clusters of 8, 85 by 4, 75 by 2, 65 by 1; float32: 138, 110, 93, 118;
-  // 48 rows bf16: 30, 23, 29, 29.  (And no block more than 120000: see a.limb.)
+  // 48 rows bf16: 30, 23, 29, 29.  (And no block more than 131000: see a.limb.)
   int cluster = 1;
   const auto rows_at_once = [&] { return std::min<int64_t>(a.rows, 2 * sm_count() / cluster); };
   while (cluster < MAX_CL && a.vocab >= 4096 * cluster &&
-         (a.vocab > 120000 * cluster || a.rows * cluster * 2 <= sm_count() ||
+         (a.vocab > 131000 * cluster || a.rows * cluster * 2 <= sm_count() ||
           (a.vocab >= 12288 * cluster && a.rows * cluster <= sm_count()) ||
           rows_at_once() * a.vocab * (int64_t)sizeof(T) > (96 << 20)))
     cluster *= 2;
@@ -1281,7 +1393,7 @@ extern "C" int gq_sample(const void* logits, int dtype, int64_t rows, int64_t vo
   const int bits = std::min(45, 62 - log2v);  // S: a term has S + 1 bits
   a.scale = (double)(1ll << bits);
   // The low limbs are below 2^limb, the high one at most 2^(S - 2 limb): 15 bits for S
-  // from 43 to 45, at most 120000 tokens a block (run() sees to that); 14 for S = 42
+  // from 43 to 45, at most 131000 tokens a block (run() sees to that); 14 for S = 42
   // (2^20 tokens in 8 blocks).  Either way a block's sum of one stays below 2^32.
   a.limb = (bits + 2) / 3;
   cudaStream_t st = as_stream(stream);
