@@ -409,9 +409,10 @@ int gq_unpack_dequant(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp,
  * gq_linear: x [tokens, n] (ldx) of dtype 0 = float32, 1 = bf16, 2 = fp16,
  * y [tokens, m] (ldy) of the same type; qw and params 16-byte aligned;
  * direct = 1 when kmap is the identity with k == n (16-bit x is then read in
- * place if it is 16-byte aligned with ldx % 8 == 0, and needs no workspace).  bits, granule and k as laid out.  Products are
- * summed in float32 in a fixed order and rounded once; float32 x runs as three
- * exact bf16 terms.  x and y must not overlap.  workspace: 256-byte aligned,
+ * place if it is 16-byte aligned with ldx % 8 == 0, and needs no workspace).
+ * bits, granule and k as laid out.  Products are summed in float32 in a fixed
+ * order and rounded once; float32 x runs as three exact bf16 terms (what lies
+ * below 2^-126 may be lost).  x and y must not overlap.  workspace: 256-byte aligned,
  * gq_linear_workspace_size(tokens, k, dtype) bytes. */
 int gq_linear_layout(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp, int bits, int sym,
                      const float* scales, const float* zeros, int64_t n_groups,

@@ -24,7 +24,7 @@ from .packing import PackedLinear
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class PreparedLinear:
     """Packed weights laid out for ``packed_matmul`` (see ``gq_linear_layout``)."""
     qweight: torch.Tensor   # laid-out codes, int32 words
@@ -130,15 +130,18 @@ def prepare_linear(p: PackedLinear) -> PreparedLinear:
 def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     """``x @ W.T`` for ``x`` [..., n] (float32, bf16 or fp16) -> [..., m] of x's type.
 
-    Products are summed in float32 (float32 x loses no bits: it runs as three
-    exact bf16 terms) and rounded once.  numpy in -> numpy out.  ``out``, if
-    given, is a contiguous tensor of the result's shape and type that does not
-    share memory with ``x``."""
+    Products are summed in float32 (float32 x runs as three exact bf16 terms:
+    it loses no bits above 2^-126) and rounded once.  numpy in -> numpy out.
+    ``out``, if given, is a contiguous tensor of the result's shape and type
+    that does not share memory with ``x``.  There is no gradient: an ``x`` that
+    asks for one is refused."""
     dt = _DTYPES.get(getattr(x, "dtype", None))
     if dt is None:
         if A.is_host(x):
             return A.like_input(packed_matmul(A.to_device(x), w), x)
         raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("packed_matmul has no gradient: call it under torch.no_grad()")
     n, m, dev = w.n, w.m, x.get_device()
     if x.dim() < 1 or x.shape[-1] != n:
         raise ValueError(f"x must be [..., {n}], got {tuple(x.shape)}")

@@ -115,6 +115,7 @@ class DecoderBlock(torch.nn.Module):
         h = self.post_attention_layernorm(x)
         return x + self.down_proj(F.silu(self.gate_proj(h)) * self.up_proj(h))
 
+    @torch.no_grad()
     def decode(self, x, cache: "KVCache", plan: rotary.RotaryPlan):
         """``forward`` for x [B, S, hidden] that follows the positions already
         in ``cache``, whose keys and values it extends."""

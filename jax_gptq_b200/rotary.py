@@ -168,6 +168,20 @@ def _results(q, k, out):
     return oq, ok
 
 
+class _Turned(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, plan, transpose):
+        ctx.save_for_backward(positions, plan.turns)
+        ctx.plan, ctx.transpose = plan, transpose
+        return apply_rotary(q, k, positions, plan, transpose=transpose)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        positions, _ = ctx.saved_tensors
+        dq, dk = apply_rotary(gq, gk, positions, ctx.plan, transpose=not ctx.transpose)
+        return dq, dk, None, None, None
+
+
 def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
                  plan: RotaryPlan, out=None, transpose: bool = False):
     """Queries [B, heads, S, head_dim] and keys [B, kv_heads, S, head_dim]
@@ -176,8 +190,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
 
     ``positions``: int64 or int32, [S] or [B, S], any values.  ``k`` may be
     None.  ``out``: a pair of tensors to write, which may be ``(q, k)``
-    themselves.  ``transpose`` turns back: the gradient with respect to the
-    input is ``apply_rotary(grad, ..., transpose=True)``."""
+    themselves (then without gradients).  ``transpose`` turns back, which is
+    the gradient's map: gradients flow to q and k through a second call."""
     dt = _DTYPES.get(q.dtype)
     if dt is None:
         raise ValueError(f"q must be float32, bfloat16 or float16, got {q.dtype}")
@@ -194,6 +208,10 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         if kb != b or ks != s:
             raise ValueError(f"q and k must have one batch and length, got {tuple(q.shape)} and "
                              f"{tuple(k.shape)}")
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+        if out is not None:
+            raise ValueError("out takes no gradients: call it under torch.no_grad()")
+        return _Turned.apply(q, k, positions, plan, transpose)
     pdim = positions.dim()
     if positions.dtype not in _POSITIONS or not 1 <= pdim <= 2 or positions.shape[-1] != s or \
             (pdim == 2 and positions.shape[0] != b):

@@ -53,7 +53,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     e >= min_p.  The most likely token always stays.  The result is the
     smallest index at which the running sum of the kept e exceeds u times their
     total.  ``temperature`` 0 takes the first largest logit.  NaN and -inf
-    logits are never taken; a row with nothing else gives -1 and -inf."""
+    logits are never taken; a row with nothing else gives -1 and -inf.  The
+    results carry no gradients."""
     dt = _DTYPES.get(logits.dtype)
     if dt is None:
         raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")

@@ -263,3 +263,14 @@ def test_refusals():
                      (dict(scales=p.scales[:-1]), "scales and zeros")):
         with pytest.raises(ValueError, match=text):
             linear.prepare_linear(broken(**kw))
+
+
+def test_gradients_are_refused():
+    p, w = _packed(40, 256, 64, 4, False, 8, act_order=False)
+    x = _x((5, 256), torch.bfloat16, 1).requires_grad_()
+    lin = linear.QuantLinear(p)
+    with pytest.raises(ValueError, match="no gradient"):
+        lin(x)
+    with torch.no_grad():
+        want = lin(x)
+    assert torch.equal(lin(x.detach()), want)

@@ -193,3 +193,38 @@ def test_refusals():
         rotary.apply_rotary(wide[:, :, :9], None, pos, plan, out=(wide[:, :, 1:], None))
     with pytest.raises(ValueError, match="share memory"):
         rotary.apply_rotary(q, q.clone(), pos, plan, out=(wide[:, :, :9], wide[:, :, 1:]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("kv_heads", [0, 2])
+def test_gradients(kv_heads, interleaved, dtype):
+    """Against the formula's, and against differences: the map is linear, so
+    f(q + v) - f(q) = f(v), and <w, f(v)> = <gradient, v> up to the tolerances
+    of f(v) and of the gradient."""
+    plan = rotary.rotary_plan(24, rotary_dim=12, interleaved=interleaved)
+    inv, _ = rotary.rotary_frequencies(12)
+    pos = torch.randint(0, 4000, (2, 19), device="cuda", dtype=torch.int32)
+    q = _heads(2, 6, 19, 24, dtype, 5).requires_grad_()
+    k = _heads(2, kv_heads, 19, 24, dtype, 6).requires_grad_() if kv_heads else None
+    oq, ok = rotary.apply_rotary(q, k, pos, plan)
+    leaves, outs = ([q, k], [oq, ok]) if kv_heads else ([q], [oq])
+    ws = [torch.randn_like(o) for o in outs]
+    grads = torch.autograd.grad(outs, leaves, ws)
+    fi = torch.finfo(dtype)
+    for x, w, g in zip(leaves, ws, grads):
+        _check(g, w, pos, plan, inv, transpose=True)
+        v = torch.randn_like(x)
+        with torch.no_grad():
+            fv = rotary.apply_rotary(v, None, pos, plan)[0]
+        room = 0.0
+        for a, b, back in ((v, w, False), (w, v, True)):
+            ref, tol = _reference(a, pos, plan, inv, back)
+            tol = tol * (1 + fi.eps) + fi.eps / 2 * ref.abs() + fi.smallest_normal * fi.eps
+            room += float((b.double().abs() * tol).sum())
+        assert abs(float((w.double() * fv.double()).sum() - (g.double() * v.double()).sum())) <= room
+    # one output alone, an expanded gradient
+    gq, = torch.autograd.grad(rotary.apply_rotary(q, k, pos, plan)[0].sum(), q)
+    _check(gq, torch.ones_like(q), pos, plan, inv, transpose=True)
+    with pytest.raises(ValueError, match="out takes no gradients"):
+        rotary.apply_rotary(q, None, pos, plan, out=(torch.empty_like(q), None))
