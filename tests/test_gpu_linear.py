@@ -106,6 +106,20 @@ def test_every_width(bits, sym, dtype):
         _check(linear.packed_matmul(x, pl), x, w, pl)
 
 
+@pytest.mark.parametrize("t", [1, 5, 8, 27])
+@pytest.mark.parametrize("n", [2048, 4000, 16384])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_and_long_sums(dtype, n, t):
+    """Clusters of 2 to 8 CTAs share a sum, with x in place and gathered."""
+    for act_order in (False, True):
+        p, w = _packed(37, n, 128, 4, False, n + t, act_order=act_order)
+        pl = linear.prepare_linear(p)
+        x = _x((t, n), dtype, t)
+        y = linear.packed_matmul(x, pl)
+        _check(y, x, w, pl)
+        assert torch.equal(y, linear.packed_matmul(x, pl))
+
+
 @pytest.mark.parametrize("t", [1, 12, 140])
 def test_groups_of_uneven_sizes(t):
     p, w = _packed(40, 700, 50, 4, False, 3, act_order=False, uneven=True)
