@@ -72,6 +72,10 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors may share memory.  Views side by side in one buffer
     (heads of a joint projection, columns of one matrix) are told apart by the
     outer dimensions they have in common; what is not decided counts as shared."""
+    sa, sb = a.untyped_storage(), b.untyped_storage()
+    pa, pb = sa.data_ptr(), sb.data_ptr()
+    if pa + sa.nbytes() <= pb or pb + sb.nbytes() <= pa:  # nearly always, and quickly told
+        return False
     if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
         return False
     da = sorted((s * a.element_size(), n) for n, s in zip(a.shape, a.stride()) if n > 1)
@@ -108,6 +112,8 @@ def _apart(a, b, da, db, common) -> bool:
 def distinct_elements(t: torch.Tensor) -> bool:
     """Whether no two elements of ``t`` share memory, judged by its strides:
     each is at least the span of the ones below it."""
+    if t.is_contiguous():
+        return True
     span = 1
     for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
         if s < span:

@@ -527,8 +527,11 @@ int gq_linear(const uint32_t* qw, const float* params, const int32_t* kmap, int6
     a.x = xp;
     a.ldx = k;
   }
-  // the few-token form up to one CTA's columns, the tcgen05 form above
-  if (a.cols > (dtype == 0 ? 24 : 32))
+  // The few-token form up to one CTA's columns, the tcgen05 form above, and from 25
+  // on where its row tiles alone fill the SMs.  32 against 33 tokens: 4096 x 4096 9.4
+  // and 12.4 us, 11008 x 4096 23.4 and 22.6, 28672 x 8192 94 and 71.
+  const int few = dtype == 0 || m >= 148 * 128 ? 24 : 32;
+  if (a.cols > few)
     return lin::run_many(qw, params, m, k, bits, granule, a.x, a.ldx, dtype, tokens, y, ldy, st);
   const bool dep = !in_place;
   if (bits <= 4) {

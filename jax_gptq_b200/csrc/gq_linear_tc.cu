@@ -739,7 +739,6 @@ int run_typed(const uint16_t* x, int64_t ldx, int64_t k, int granule, const Para
     if (p.tokens <= 32) return run_tile<WIDTH, T, 96, 1>(x, ldx, k, granule, p, st);
     return run_tile<WIDTH, T, 96, 2>(x, ldx, k, granule, p, st);
   } else {
-    if (p.tokens <= 32) return run_tile<WIDTH, T, 32, 1>(x, ldx, k, granule, p, st);
     if (p.tokens <= 64) return run_tile<WIDTH, T, 64, 1>(x, ldx, k, granule, p, st);
     if (p.tokens <= 128) return run_tile<WIDTH, T, 128, 1>(x, ldx, k, granule, p, st);
     // 256 columns and the 8-bit codes' stages together exceed shared memory

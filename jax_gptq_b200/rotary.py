@@ -160,7 +160,7 @@ def _results(q, k, out):
             raise ValueError(f"out of {name} must be like it, with contiguous components")
         if not A.distinct_elements(o):
             raise ValueError(f"out of {name} has elements that share memory")
-        same = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
+        same = o is x or (o.data_ptr() == x.data_ptr() and o.stride() == x.stride())
         if not same and A.overlap(o, x):
             raise ValueError(f"out of {name} partly shares memory with it")
     if k is not None and (A.overlap(oq, ok) or A.overlap(oq, k) or A.overlap(ok, q)):

@@ -120,6 +120,14 @@ def test_few_rows_and_long_sums(dtype, n, t):
         assert torch.equal(y, linear.packed_matmul(x, pl))
 
 
+@pytest.mark.parametrize("t", [8, 24, 25, 32])
+def test_many_rows(t):
+    p, w = _packed(18950, 256, 128, 4, False, t, act_order=False)
+    pl = linear.prepare_linear(p)
+    x = _x((t, 256), torch.bfloat16, t)
+    _check(linear.packed_matmul(x, pl), x, w, pl)
+
+
 @pytest.mark.parametrize("t", [1, 12, 140])
 def test_groups_of_uneven_sizes(t):
     p, w = _packed(40, 700, 50, 4, False, 3, act_order=False, uneven=True)

@@ -216,6 +216,22 @@ def test_logprob_is_what_the_evaluation_scores():
     assert abs(nll + float(got.logprobs.double().sum())) <= 1e-5 * abs(nll)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [9000, 40000])
+def test_rows_do_not_depend_on_the_batch(vocab, dtype):
+    """The split of a row over blocks follows the number of rows; whole-number
+    sums make the results the same for every split."""
+    z, u = _logits(300, vocab, dtype, vocab)
+    settings = dict(temperature=0.5 + torch.rand(300, device="cuda"),
+                    top_k=torch.where(u < 0.5, 0, 1 + (u * 3000)).int(),
+                    top_p=torch.where(u < 0.2, 1.0, 0.5 + u / 2), min_p=torch.where(u > 0.7, 0.01, 0.0))
+    all_at_once = sampling.sample_tokens(z, u, **settings)
+    for n in (1, 20, 100):
+        some = sampling.sample_tokens(z[:n], u[:n], **{k: v[:n] for k, v in settings.items()})
+        assert torch.equal(some.tokens, all_at_once.tokens[:n])
+        assert torch.equal(some.logprobs, all_at_once.logprobs[:n])
+
+
 @pytest.mark.parametrize("rows,vocab", [(150, 110000), (2, 1 << 20)])
 def test_flat_rows(rows, vocab):
     """Nearly all of a block's tokens in one cell: its sums have to have room for
