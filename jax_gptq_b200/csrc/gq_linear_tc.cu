@@ -34,6 +34,12 @@
 // leaves its sums in its own shared memory and adds up its share of the columns
 // over the cluster in rank order.  No load uses multicast.
 //
+// Bound: 2048 tokens through 11008 x 4096 take 192 us, 960 TFLOP/s, where cuBLAS on
+// weights already decoded reaches 1426 in a long run and 1686 in a burst: the roles
+// take turns at tensor memory, which three accumulators and two decoded blocks fill.
+// Few tokens (37 float32 ones through 4096 x 4096: 14 us and 3 of the gather) are a
+// chain of about 1600 cycles a block of K.
+//
 // Every wait is bounded (gq_set_wait_limit_ns): one that expires makes all roles
 // leave their loops and records GQ_DEVERR_TIMEOUT, read by gq_device_status().
 #include <cuda.h>
@@ -700,6 +706,13 @@ int launch(const CUtensorMap& map, const CUtensorMap& map_w, const Params& p, cu
   return check_launch("gq_linear many-token product");
 }
 
+// CTAs that K can be split over: each keeps 4 blocks.
+inline int most_parts(int nkc) {
+  int parts = 1;
+  while (parts < 8 && nkc >= parts * 2 * 4) parts *= 2;
+  return parts;
+}
+
 template <int WIDTH, typename T, int N, int PARTS>
 int run_tile(const uint16_t* x, int64_t ldx, int64_t k, int granule, Params p, cudaStream_t st) {
   constexpr int SPLIT = std::is_same<T, float>::value ? 3 : 1;
@@ -724,23 +737,34 @@ int run_tile(const uint16_t* x, int64_t ldx, int64_t k, int granule, Params p, c
   p.nt = (int)ceil_div(p.tokens, TOK);
   const int64_t tiles = (int64_t)p.mt * p.nt;
   GQ_REQUIRE(tiles < (1ll << 31), "gq_linear: too many tiles");
-  // split K over a cluster while that fills idle SMs and leaves 4 blocks each
+  // Split K over a cluster while that fills idle SMs and leaves 4 blocks each.  Of
+  // clusters of 8, one CTA an SM, 14 run at once: 128 tokens through 2048 x 8192 (16
+  // tiles) take 28.4 us by 8 and 20.7 by 4, through 1792 x 8192 17.0 by 8.
+  const int most = most_parts(p.nkc);
   p.split = 1;
-  while (p.split < 8 && tiles * p.split * 2 <= sm_count() && p.nkc >= p.split * 2 * 4) p.split *= 2;
+  while (p.split < most && tiles * p.split * 2 <= (p.split == 4 ? 112 : sm_count())) p.split *= 2;
   if (granule == 128) return launch<WIDTH, T, N, PARTS, 128>(map, map_w, p, st);
   if (granule == 64) return launch<WIDTH, T, N, PARTS, 64>(map, map_w, p, st);
   return launch<WIDTH, T, N, PARTS, 32>(map, map_w, p, st);
 }
 
+// The columns of x per tile: what a CTA can hold, or less where narrower tiles, split
+// along K as far as it goes, still take no more than half the SMs (more of them meet
+// the limit on clusters above: 128 tokens through 1024 x 8192 16.6 us, by 64 columns
+// 24.1).  255 tokens through 276 x 512 at granule 32: 19.3 us by 256 columns, 11.7 by
+// 64; 61 float32 tokens through 96 x 4608: 20.2 by 192, 16.3 by 96.
 template <int WIDTH, typename T>
 int run_typed(const uint16_t* x, int64_t ldx, int64_t k, int granule, const Params& p,
               cudaStream_t st) {
+  auto idle = [&](int tokens) {  // tiles of so many tokens leave SMs idle
+    return ceil_div(p.m, BM) * ceil_div(p.tokens, tokens) * most_parts(p.nkc) <= sm_count() / 2;
+  };
   if constexpr (std::is_same<T, float>::value) {  // three columns a token
-    if (p.tokens <= 32) return run_tile<WIDTH, T, 96, 1>(x, ldx, k, granule, p, st);
+    if (p.tokens <= 32 || idle(32)) return run_tile<WIDTH, T, 96, 1>(x, ldx, k, granule, p, st);
     return run_tile<WIDTH, T, 96, 2>(x, ldx, k, granule, p, st);
   } else {
-    if (p.tokens <= 64) return run_tile<WIDTH, T, 64, 1>(x, ldx, k, granule, p, st);
-    if (p.tokens <= 128) return run_tile<WIDTH, T, 128, 1>(x, ldx, k, granule, p, st);
+    if (p.tokens <= 64 || idle(64)) return run_tile<WIDTH, T, 64, 1>(x, ldx, k, granule, p, st);
+    if (p.tokens <= 128 || idle(128)) return run_tile<WIDTH, T, 128, 1>(x, ldx, k, granule, p, st);
     // 256 columns and the 8-bit codes' stages together exceed shared memory
     return run_tile<WIDTH, T, WIDTH == 4 ? 128 : 96, 2>(x, ldx, k, granule, p, st);
   }

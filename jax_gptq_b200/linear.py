@@ -178,7 +178,9 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
 
 
 class QuantLinear(torch.nn.Module):
-    """A bias-free linear on packed weights (inference only)."""
+    """A bias-free linear on packed weights (inference only).  They stay on the
+    device they were laid out on and are not part of ``state_dict``: a packed
+    checkpoint keeps them."""
 
     def __init__(self, p: PackedLinear | PreparedLinear):
         super().__init__()
