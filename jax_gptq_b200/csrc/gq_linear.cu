@@ -210,11 +210,12 @@ struct Args {
 
 // One cluster: 16 rows, up to 8 NT columns; the warps of its CTAs take
 // contiguous shares of K and their sums are added in order.
-// Bound: reading the weights, in the end; now the integer pipe (7 operations for
-// 8 codes and the loop's own, 62 % busy) and the loads' latency that 24 warps an
-// SM leave bare.  1 token bf16 of 28672 x 8192: 33.3 us, 4.0 TB/s; of 11008 x 4096
-// 8.0 us, of 4096 x 4096 3.8 us, 1024 x 1024 1.9 us.  Four warps a CTA and twice
-// the CTAs take 9 to 15 us where 256 row blocks take 9; four blocks in flight spill.
+// Bound: reading the weights, in the end; now the loads' latency that 24 warps an SM
+// leave bare, most of all where a CTA begins (issue slots 48 % busy, the integer pipe
+// 45 %), and whole rounds of CTAs.  1 token bf16 of 28672 x 8192: 33.3 us, 4.0 TB/s (4.04
+// rounds); of 11008 x 4096 8.0 us, of 4096 x 4096 3.8 us, of 1024 x 1024 1.9 us.  Four
+// warps a CTA and twice the CTAs take 9 to 15 us where 256 row blocks take 9; four
+// blocks in flight spill.
 template <int WIDTH, typename T, int NT, int G>
 __global__ void __launch_bounds__(32 * WARPS, NT == 1 ? 3 : 2)
     few_kernel(Args a, int split, bool dependent) {
