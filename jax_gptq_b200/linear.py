@@ -168,7 +168,7 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     xp, wp, nbytes = x2.data_ptr(), None, 0
     if not (w.direct and dt and xp % 16 == 0 and ldx % 8 == 0):  # x is first put in order
         nbytes = lib.gq_linear_workspace_size(tokens, w.k, dt)
-        ws = A.workspace(nbytes)
+        ws = x2.new_empty(nbytes // x2.element_size())  # (a multiple of 256)
         wp = ws.data_ptr()
     status = lib.gq_linear(*w._head, xp, dt, tokens, ldx, out.data_ptr(), m, wp, nbytes,
                            A.raw_stream(dev))
