@@ -821,12 +821,15 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     const uint32_t k_before = sh.found_count;  // with cut_k: tokens of the bins before
     const int floor_bin = by_min ? (int)fmin(floor_y * 11.0 + 0.01, BINS - 2.0) : BINS - 2;
     // (top-p after top-k needs the mass of all k, though)
+    bool k_border = cut_k;  // `limit` is the k-th token's bin: top-k has a border to find
     if (limit > floor_bin && !(cut_k && by_p)) {
       tell(tid == floor_bin ? tid : -1, 0, 0, bc + hc, 0);
-      // worth it where it makes the list short; the general way needs the border's own bin
+      // worth it where it makes the list short.  All that min-p keeps then lies in bins
+      // before the k-th token's, so that top-k takes nothing of it
       if (sh.found_own <= LIST) {
         limit = floor_bin;
         through = sh.found_own;
+        k_border = false;
       }
     }
     if (limit >= 0) {
@@ -858,7 +861,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
           border_at(place, border);
         }
       } else {
-        if (cut_k) {
+        // (a list shortened by min-p can be too long all the same: it reaches a little
+        // past its bin, where many equal logits may lie)
+        if (k_border) {
           n = collect([&](float x) { return bin_of(x) == limit; });
           if (n <= LIST) {
             sorted(n);

@@ -168,6 +168,51 @@ def test_masked_infinite_and_empty_rows(dtype):
         assert got.tokens[5] == 77 and 100 <= got.tokens[6] < 103
 
 
+def _runs_past_min_p(vocab, inside, past, dtype):
+    """Rows, temperature and min_p for which `past` equal logits lie 1 part in
+    21000 of a bin (an 11th of a power of two) behind the end of min-p's bin,
+    with one logit at the top and `inside` equal ones in the bin."""
+    z = torch.full((6, vocab), -8.0, device="cuda")
+    at = torch.randperm(vocab, generator=torch.Generator().manual_seed(vocab))
+    z[:, at[0]] = 0.0
+    z[:, at[1:1 + inside]] = -0.9765625
+    z[:, at[1 + inside:1 + inside + past]] = -1.0
+    return z.to(dtype), 11 / math.log(2) / 21.001, 2.0 ** (-20.7 / 11)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab,inside,past,k", [
+    (5000, 1500, 1000, 1512), (5000, 1500, 1000, 2500), (32000, 1500, 30000, 20000),
+    (32000, 2000, 60, 2055), (128256, 1900, 100000, 90000), (128256, 10, 100000, 90000),
+    (128256, 10, 1000, 900), (5000, 1500, 1000, 1000), (5000, 2047, 1000, 3000),
+    (5000, 2048, 1000, 3000), (5000, 2100, 1000, 3000)])
+def test_min_p_before_the_border_of_top_k(vocab, inside, past, k, dtype):
+    """The list that min-p makes short enough grows too long by equal logits next
+    to its end; the k-th token lies in a later bin."""
+    z, t, mp = _runs_past_min_p(vocab, inside, past, dtype)
+    u = torch.tensor([0.0, 0.2, 0.4, 0.6, 0.8, 0.999], device="cuda")
+    got = _check(z, u, temperature=t, top_k=k, min_p=mp)
+    _check(z, u, temperature=t, min_p=mp)
+    _check(z, u, temperature=t, top_k=k)
+    _check(z, u, temperature=t, top_k=k, top_p=0.97, min_p=mp)
+    _check(z, u, temperature=t, top_p=0.999, min_p=mp)
+    one = _check(z[2:3], u[2:3], temperature=t, top_k=k, min_p=mp)
+    assert one.tokens[0] == got.tokens[2] and one.logprobs[0] == got.logprobs[2]
+
+
+@pytest.mark.parametrize("k", [3, 2500, 9000, 30000])
+def test_top_k_with_min_p_on_coarse_logits(k):
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    z = torch.randint(-40, 41, (32, 40000), generator=gen, device="cuda").to(torch.bfloat16) / 8
+    u = torch.rand((32,), generator=gen, device="cuda")
+    # every row another temperature; min_p halfway between the terms of two logits
+    t = 0.4 + 3 * torch.rand((32,), generator=gen, device="cuda").double()
+    steps = torch.randint(0, 60, (32,), generator=gen, device="cuda")
+    mp = torch.exp(-(steps.double() + 0.5) / 8 / t)
+    _check(z, u, temperature=t, top_k=k, min_p=mp)
+    _check(z.float(), u, temperature=t, top_k=k, min_p=mp)
+
+
 def test_settings_per_row():
     rows = 64
     z, u = _logits(rows, 20011, torch.float32, 5)
