@@ -419,6 +419,12 @@ int gq_linear_layout(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp, 
                      const int32_t* kmap, int64_t k, const int32_t* granule_group, int granule,
                      uint32_t* qw, float* params, int* bad, void* stream);
 int64_t gq_linear_workspace_size(int64_t tokens, int64_t k, int dtype);
+/* Which form gq_linear takes on a device of `sms` SMs (for tests; nothing is
+ * launched).  form (HOST, 10 values): all 0 = the few-token form; else columns
+ * of an MMA, MMAs side by side, CTAs along K, tiles, and slots and barriers of
+ * the rings of copied codes, decoded blocks and accumulators. */
+int gq_test_linear_form(int64_t m, int64_t k, int bits, int granule, int dtype, int64_t tokens,
+                        int sms, int64_t* form);
 int gq_linear(const uint32_t* qw, const float* params, const int32_t* kmap, int64_t m, int64_t n,
               int64_t k, int bits, int granule, int direct, const void* x, int dtype,
               int64_t tokens, int64_t ldx, void* y, int64_t ldy, void* workspace,

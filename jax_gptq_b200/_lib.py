@@ -37,6 +37,7 @@ SIGNATURES = {
                                   _P, _P, _P, _P]),
     "gq_linear_layout": (c_int, [_P, c_int64, c_int64, c_int64, c_int, c_int, _P, _P, c_int64, _P,
                                  c_int64, _P, c_int, _P, _P, _P, _P]),
+    "gq_test_linear_form": (c_int, [c_int64, c_int64, c_int, c_int, c_int, c_int64, c_int, _P]),
     "gq_linear_workspace_size": (c_int64, [c_int64, c_int64, c_int]),
     "gq_linear": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_int, c_int, c_int, _P, c_int,
                           c_int64, c_int64, _P, c_int64, _P, c_int64, _P]),

@@ -430,6 +430,11 @@ int run_typed(const Args& a, int granule, bool dependent, cudaStream_t st) {
   return run_few<WIDTH, T, 3>(a, granule, dependent, st);
 }
 
+// The columns of x that the few-token form takes: one CTA's, and 24 where the tcgen05
+// form's row tiles alone fill the SMs.  32 against 33 tokens: 4096 x 4096 9.4 and 12.4
+// us, 11008 x 4096 23.4 and 22.6, 28672 x 8192 94 and 71.
+inline int few_columns(int dtype, int64_t m) { return dtype == 0 || m >= 148 * 128 ? 24 : 32; }
+
 inline int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
 
 }  // namespace lin
@@ -472,6 +477,20 @@ int gq_linear_layout(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp, 
       scales, zeros, m, n_groups, qmin, (float)((1 << bits) - 1), granule_group, ngran,
       reinterpret_cast<float2*>(params), total, bad);
   return check_launch("gq_linear_layout params");
+}
+
+int gq_test_linear_form(int64_t m, int64_t k, int bits, int granule, int dtype, int64_t tokens,
+                        int sms, int64_t* form) {
+  using namespace gq;
+  GQ_REQUIRE(form != nullptr && m >= 1 && m < (1ll << 31) && tokens >= 1 && tokens < (1ll << 29) &&
+                 k >= 1 && k < (1ll << 31) && k % lin::KC == 0 && bits >= 1 && bits <= 8 &&
+                 (granule == 32 || granule == 64 || granule == 128) && dtype >= 0 && dtype <= 2 &&
+                 sms >= 1,
+             "gq_test_linear_form: bad argument");
+  for (int i = 0; i < 10; ++i) form[i] = 0;
+  if (tokens * (dtype == 0 ? 3 : 1) > lin::few_columns(dtype, m))
+    lin::many_form(m, k, bits, granule, dtype, tokens, sms, form);
+  return GQ_OK;
 }
 
 int64_t gq_linear_workspace_size(int64_t tokens, int64_t k, int dtype) {
@@ -533,11 +552,7 @@ int gq_linear(const uint32_t* qw, const float* params, const int32_t* kmap, int6
     a.x = xp;
     a.ldx = k;
   }
-  // The few-token form up to one CTA's columns, the tcgen05 form above, and from 25
-  // on where its row tiles alone fill the SMs.  32 against 33 tokens: 4096 x 4096 9.4
-  // and 12.4 us, 11008 x 4096 23.4 and 22.6, 28672 x 8192 94 and 71.
-  const int few = dtype == 0 || m >= 148 * 128 ? 24 : 32;
-  if (a.cols > few)
+  if (a.cols > lin::few_columns(dtype, m))
     return lin::run_many(qw, params, m, k, bits, granule, a.x, a.ldx, dtype, tokens, y, ldy, st);
   const bool dep = !in_place;
   if (bits <= 4) {

@@ -107,6 +107,11 @@ __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 int run_many(const uint32_t* qw, const float* params, int64_t m, int64_t k, int bits, int granule,
              const uint16_t* x, int64_t ldx, int dtype, int64_t tokens, void* y, int64_t ldy,
              cudaStream_t st);
+// Its choice on a device of `sms` SMs: columns of an MMA, MMAs side by side, CTAs along K,
+// tiles, and the slots and barriers of its three rings (copied codes, decoded blocks,
+// accumulators).
+void many_form(int64_t m, int64_t k, int bits, int granule, int dtype, int64_t tokens, int sms,
+               int64_t* form);
 
 }  // namespace lin
 }  // namespace gq

@@ -94,6 +94,15 @@ struct Cfg {
   static constexpr int SCALES = BM * (KC / G) * 8;         // and its scales and offsets
   static constexpr int WSTAGE = CODES + SCALES;
   static constexpr int WSTAGES = TILE > 192 ? (G < 128 ? 2 : 3) : 4;
+  // Where two groups of warps take a ring's slots in turn, a group meets a slot of an
+  // odd ring only every second time round.  A wait for a phase returns at once while the
+  // phase before it is still open, so a group that never waited for that one could take
+  // a slot too early.  Odd rings therefore have two barriers a slot, used in turn: a
+  // barrier's last use is then the same group's, which has waited for it.
+  static constexpr int barriers(int slots) { return slots % 2 ? 2 * slots : slots; }
+  static constexpr int W_FULL = barriers(WSTAGES);    // decoders: copied codes
+  static constexpr int A_EMPTY = barriers(ASTAGES);   // decoders: room for a decoded block
+  static constexpr int T_FULL = PARTS == 2 ? barriers(ACCS) : ACCS;  // accumulating groups
   static constexpr int PER = PARTS == 2 ? N : N / 2;  // columns per accumulating thread
   static constexpr int LD = PER % 16 == 0 ? 16 : 8;
   static constexpr int A0 = ACCS * N;                 // first tensor-memory column of the weights
@@ -313,9 +322,9 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  __shared__ uint64_t x_full[C::STAGES], x_empty[C::STAGES], a_full[C::ASTAGES], a_empty[C::ASTAGES];
-  __shared__ uint64_t w_full[C::WSTAGES], w_empty[C::WSTAGES];
-  __shared__ uint64_t t_full[C::ACCS], t_empty[C::ACCS], done;
+  __shared__ uint64_t x_full[C::STAGES], x_empty[C::STAGES], a_full[C::ASTAGES], a_empty[C::A_EMPTY];
+  __shared__ uint64_t w_full[C::W_FULL], w_empty[C::WSTAGES];
+  __shared__ uint64_t t_full[C::T_FULL], t_empty[C::ACCS], done;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -326,18 +335,12 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       mbar_init(&x_full[s], 1);
       mbar_init(&x_empty[s], 1);
     }
-    for (int s = 0; s < C::ASTAGES; ++s) {
-      mbar_init(&a_full[s], 4);  // the decoding warps of a block
-      mbar_init(&a_empty[s], 1);
-    }
-    for (int s = 0; s < C::WSTAGES; ++s) {
-      mbar_init(&w_full[s], 1);
-      mbar_init(&w_empty[s], 4);  // the decoding warps of a block
-    }
-    for (int h = 0; h < C::ACCS; ++h) {
-      mbar_init(&t_full[h], 1);
-      mbar_init(&t_empty[h], PARTS == 2 ? 4 : 8);  // the warps that read it
-    }
+    for (int s = 0; s < C::ASTAGES; ++s) mbar_init(&a_full[s], 4);  // the decoding warps of a block
+    for (int s = 0; s < C::A_EMPTY; ++s) mbar_init(&a_empty[s], 1);
+    for (int s = 0; s < C::W_FULL; ++s) mbar_init(&w_full[s], 1);
+    for (int s = 0; s < C::WSTAGES; ++s) mbar_init(&w_empty[s], 4);  // the decoding warps of a block
+    for (int h = 0; h < C::T_FULL; ++h) mbar_init(&t_full[h], 1);
+    for (int h = 0; h < C::ACCS; ++h) mbar_init(&t_empty[h], PARTS == 2 ? 4 : 8);  // the warps that read it
     mbar_init(&done, 1);
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -381,7 +384,8 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         const uint32_t b_base = smem_u32(smem) + s * C::XSTAGE;
         const uint32_t a_base = tmem + C::A0 + as * A_COLS;
         uint64_t* const x_done = &x_empty[s];
-        uint64_t* const a_done = &a_empty[as];
+        // (every second time round a ring, an odd one's second barriers)
+        uint64_t* const a_done = &a_empty[as + (C::A_EMPTY > C::ASTAGES && aphase ? C::ASTAGES : 0)];
         if (++s == C::STAGES) {
           s = 0;
           phase ^= 1;
@@ -398,6 +402,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int cur = acc;
+            uint64_t* const t_done = &t_full[cur + (C::T_FULL > C::ACCS && tphase ? C::ACCS : 0)];
             if (++acc == C::ACCS) {
               acc = 0;
               tphase ^= 1;
@@ -414,7 +419,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
               umma(leader, tmem + cur * N, a_base + kk * 8,
                    make_desc(b_base + (kk / 4) * C::BOX + h * N * 128 + (kk % 4) * 32), IDESC, i > 0);
             }
-            umma_commit(leader, &t_full[cur]);
+            umma_commit(leader, t_done);
           }
         }
         if (!ok) break;
@@ -427,6 +432,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       // copies by tensor map: x; codes and scales of 8 blocks of 16 rows (rows
       // past the last block read as zeros)
       const int stages = warp == 0 ? C::STAGES : C::WSTAGES;
+      const int fulls = warp == 0 ? C::STAGES : C::W_FULL;
       uint64_t* fb = warp == 0 ? x_full : w_full;
       uint64_t* eb = warp == 0 ? x_empty : w_empty;
       int s = 0, loads = 0;
@@ -437,16 +443,17 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         for (int c = c0; c < c1; ++c) {
           if (!(ok = mbar_wait_warp(&eb[s], phase ^ 1, abort_flag))) break;
           if (lane == 0) {
+            uint64_t* const full = &fb[s + (fulls > stages && phase ? stages : 0)];
             if (warp == 0) {
               uint8_t* dst = smem + s * C::XSTAGE;
-              mbar_expect_tx(&fb[s], C::XSTAGE);
-              tma_load_2d(&map_x, &fb[s], dst, c * KC, col);
-              tma_load_2d(&map_x, &fb[s], dst + C::BOX, c * KC + 64, col);
+              mbar_expect_tx(full, C::XSTAGE);
+              tma_load_2d(&map_x, full, dst, c * KC, col);
+              tma_load_2d(&map_x, full, dst + C::BOX, c * KC + 64, col);
             } else {
               uint8_t* dst = smem + C::W0 + s * C::WSTAGE;
-              mbar_expect_tx(&fb[s], C::WSTAGE);
-              tma_load_3d(&map_w, &fb[s], dst, 0, c, rb0);
-              tma_load_3d(&map_s, &fb[s], dst + C::CODES, 0, c, rb0);
+              mbar_expect_tx(full, C::WSTAGE);
+              tma_load_3d(&map_w, full, dst, 0, c, rb0);
+              tma_load_3d(&map_s, full, dst + C::CODES, 0, c, rb0);
             }
           }
           ++loads;
@@ -466,8 +473,8 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         }
       }
       if (!ok && lane == 0)
-        for (int i = 0; i < stages; ++i) {
-          const int issued = loads / stages + (i < loads % stages);
+        for (int i = 0; i < fulls; ++i) {
+          const int issued = loads / fulls + (i < loads % fulls);
           if (issued > 0) mbar_drain(&fb[i], (issued - 1) & 1);
         }
     }
@@ -486,7 +493,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
       for (int c = c0; c < c1; ++c, ++n) {
         if ((n & 1) != mine) continue;
         const int ws = n % C::WSTAGES, as = n % C::ASTAGES;
-        if (!(ok = mbar_wait_warp(&w_full[ws], (n / C::WSTAGES) & 1, abort_flag))) break;
+        if (!(ok = mbar_wait_warp(&w_full[n % C::W_FULL], (n / C::W_FULL) & 1, abort_flag))) break;
         const uint8_t* stage = smem + C::W0 + ws * C::WSTAGE;
         const uint4* codes = reinterpret_cast<const uint4*>(stage) + rt * LPR;
         const float2* sc = reinterpret_cast<const float2*>(stage + C::CODES) +
@@ -499,7 +506,10 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         for (int i = 0; i < GPC; ++i) coff[i] = sc[i * ROWS].y;
         __syncwarp();
         if (lane == 0) mbar_arrive(&w_empty[ws]);
-        if (!(ok = mbar_wait_warp(&a_empty[as], ((n / C::ASTAGES) & 1) ^ 1, abort_flag))) break;
+        // the MMAs of block n - ASTAGES are over (the first blocks have room at once)
+        const uint32_t room = n + (C::A_EMPTY - C::ASTAGES);
+        if (!(ok = mbar_wait_warp(&a_empty[room % C::A_EMPTY], ((room / C::A_EMPTY) & 1) ^ 1, abort_flag)))
+          break;
         fence_after();
         const uint32_t dst = tmem + lanes + C::A0 + as * A_COLS;
 #pragma unroll
@@ -560,7 +570,7 @@ many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         // half of the columns
         const uint32_t st = PARTS == 2 ? 2 * u + part : u;  // number of the step
         const uint32_t buf = st % C::ACCS;
-        ok = mbar_wait_warp(&t_full[buf], (st / C::ACCS) & 1, abort_flag);
+        ok = mbar_wait_warp(&t_full[st % C::T_FULL], (st / C::T_FULL) & 1, abort_flag);
         ++u;
         if (!ok) break;
         fence_after();
@@ -713,6 +723,37 @@ inline int most_parts(int nkc) {
   return parts;
 }
 
+// Split K over a cluster while that fills idle SMs and leaves 4 blocks each.  Of
+// clusters of 8, one CTA an SM, 14 run at once: 128 tokens through 2048 x 8192 (16
+// tiles) take 28.4 us by 8 and 20.7 by 4, through 1792 x 8192 17.0 by 8.
+inline int choose_split(int64_t tiles, int nkc, int sms) {
+  const int most = most_parts(nkc);
+  int split = 1;
+  while (split < most && tiles * split * 2 <= (split == 4 ? 112 : sms)) split *= 2;
+  return split;
+}
+
+struct Tile {
+  int n, parts;
+  int tokens(int dtype) const { return n * parts / (dtype == 0 ? 3 : 1); }
+};
+
+// The columns of x per tile: what a CTA can hold, or less where narrower tiles, split
+// along K as far as it goes, still take no more than half the SMs (more of them meet
+// the limit on clusters above: 128 tokens through 1024 x 8192 16.6 us, by 64 columns
+// 24.1).  255 tokens through 276 x 512 at granule 32: 19.3 us by 256 columns, 11.7 by
+// 64; 61 float32 tokens through 96 x 4608: 20.2 by 192, 16.3 by 96.
+inline Tile choose_tile(int width, int dtype, int64_t m, int64_t tokens, int nkc, int sms) {
+  auto fits = [&](int each) {  // all in one tile, or tiles of so many tokens leave SMs idle
+    return tokens <= each || ceil_div(m, BM) * ceil_div(tokens, each) * most_parts(nkc) <= sms / 2;
+  };
+  if (dtype == 0) return {96, fits(32) ? 1 : 2};  // three columns a token
+  if (fits(64)) return {64, 1};
+  if (fits(128)) return {128, 1};
+  // 256 columns and the 8-bit codes' stages together exceed shared memory
+  return {width == 4 ? 128 : 96, 2};
+}
+
 template <int WIDTH, typename T, int N, int PARTS>
 int run_tile(const uint16_t* x, int64_t ldx, int64_t k, int granule, Params p, cudaStream_t st) {
   constexpr int SPLIT = std::is_same<T, float>::value ? 3 : 1;
@@ -737,42 +778,65 @@ int run_tile(const uint16_t* x, int64_t ldx, int64_t k, int granule, Params p, c
   p.nt = (int)ceil_div(p.tokens, TOK);
   const int64_t tiles = (int64_t)p.mt * p.nt;
   GQ_REQUIRE(tiles < (1ll << 31), "gq_linear: too many tiles");
-  // Split K over a cluster while that fills idle SMs and leaves 4 blocks each.  Of
-  // clusters of 8, one CTA an SM, 14 run at once: 128 tokens through 2048 x 8192 (16
-  // tiles) take 28.4 us by 8 and 20.7 by 4, through 1792 x 8192 17.0 by 8.
-  const int most = most_parts(p.nkc);
-  p.split = 1;
-  while (p.split < most && tiles * p.split * 2 <= (p.split == 4 ? 112 : sm_count())) p.split *= 2;
+  p.split = choose_split(tiles, p.nkc, sm_count());
   if (granule == 128) return launch<WIDTH, T, N, PARTS, 128>(map, map_w, p, st);
   if (granule == 64) return launch<WIDTH, T, N, PARTS, 64>(map, map_w, p, st);
   return launch<WIDTH, T, N, PARTS, 32>(map, map_w, p, st);
 }
 
-// The columns of x per tile: what a CTA can hold, or less where narrower tiles, split
-// along K as far as it goes, still take no more than half the SMs (more of them meet
-// the limit on clusters above: 128 tokens through 1024 x 8192 16.6 us, by 64 columns
-// 24.1).  255 tokens through 276 x 512 at granule 32: 19.3 us by 256 columns, 11.7 by
-// 64; 61 float32 tokens through 96 x 4608: 20.2 by 192, 16.3 by 96.
 template <int WIDTH, typename T>
 int run_typed(const uint16_t* x, int64_t ldx, int64_t k, int granule, const Params& p,
               cudaStream_t st) {
-  auto idle = [&](int tokens) {  // tiles of so many tokens leave SMs idle
-    return ceil_div(p.m, BM) * ceil_div(p.tokens, tokens) * most_parts(p.nkc) <= sm_count() / 2;
-  };
-  if constexpr (std::is_same<T, float>::value) {  // three columns a token
-    if (p.tokens <= 32 || idle(32)) return run_tile<WIDTH, T, 96, 1>(x, ldx, k, granule, p, st);
+  constexpr int DTYPE = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 2 : 1;
+  const Tile t = choose_tile(WIDTH, DTYPE, p.m, p.tokens, p.nkc, sm_count());
+  if constexpr (DTYPE == 0) {
+    if (t.parts == 1) return run_tile<WIDTH, T, 96, 1>(x, ldx, k, granule, p, st);
     return run_tile<WIDTH, T, 96, 2>(x, ldx, k, granule, p, st);
   } else {
-    if (p.tokens <= 64 || idle(64)) return run_tile<WIDTH, T, 64, 1>(x, ldx, k, granule, p, st);
-    if (p.tokens <= 128 || idle(128)) return run_tile<WIDTH, T, 128, 1>(x, ldx, k, granule, p, st);
-    // 256 columns and the 8-bit codes' stages together exceed shared memory
-    return run_tile<WIDTH, T, WIDTH == 4 ? 128 : 96, 2>(x, ldx, k, granule, p, st);
+    if (t.parts == 2) return run_tile<WIDTH, T, WIDTH == 4 ? 128 : 96, 2>(x, ldx, k, granule, p, st);
+    if (t.n == 64) return run_tile<WIDTH, T, 64, 1>(x, ldx, k, granule, p, st);
+    return run_tile<WIDTH, T, 128, 1>(x, ldx, k, granule, p, st);
   }
+}
+
+// What gq_test_linear_form tells of a configuration.
+template <int WIDTH, int N, int PARTS>
+void describe(int granule, int64_t* form) {
+  auto put = [&](auto c) {
+    using C = decltype(c);
+    const int rings[] = {C::WSTAGES, C::W_FULL, C::ASTAGES, C::A_EMPTY, C::ACCS, C::T_FULL};
+    for (int v : rings) *form++ = v;
+  };
+  if (granule == 128) put(Cfg<WIDTH, N, PARTS, 128>{});
+  else if (granule == 64) put(Cfg<WIDTH, N, PARTS, 64>{});
+  else put(Cfg<WIDTH, N, PARTS, 32>{});
 }
 
 }  // namespace lintc
 
 namespace lin {
+
+void many_form(int64_t m, int64_t k, int bits, int granule, int dtype, int64_t tokens, int sms,
+               int64_t* form) {
+  using namespace lintc;
+  const int width = bits <= 4 ? 4 : 8, nkc = (int)(k / KC);
+  const Tile t = choose_tile(width, dtype, m, tokens, nkc, sms);
+  const int64_t tiles = ceil_div(m, BM) * ceil_div(tokens, t.tokens(dtype));
+  form[0] = t.n;
+  form[1] = t.parts;
+  form[2] = choose_split(tiles, nkc, sms);
+  form[3] = tiles;
+  form += 4;
+  if (t.parts == 1) {
+    if (t.n == 64) width == 4 ? describe<4, 64, 1>(granule, form) : describe<8, 64, 1>(granule, form);
+    else if (t.n == 96) width == 4 ? describe<4, 96, 1>(granule, form) : describe<8, 96, 1>(granule, form);
+    else width == 4 ? describe<4, 128, 1>(granule, form) : describe<8, 128, 1>(granule, form);
+  } else if (t.n == 96) {
+    width == 4 ? describe<4, 96, 2>(granule, form) : describe<8, 96, 2>(granule, form);
+  } else {
+    describe<4, 128, 2>(granule, form);
+  }
+}
 
 int run_many(const uint32_t* qw, const float* params, int64_t m, int64_t k, int bits, int granule,
              const uint16_t* x, int64_t ldx, int dtype, int64_t tokens, void* y, int64_t ldy,

@@ -2,6 +2,7 @@
 and the refusals of the C entry points (nothing is launched)."""
 
 import ctypes
+import random
 
 import numpy as np
 import pytest
@@ -80,3 +81,81 @@ def test_layout_refuses_before_launching(kw, text):
     a.update(kw)
     assert _lib.lib().gq_linear_layout(*a.values()) == _lib.GQ_EINVAL
     assert text in _lib.lib().gq_last_error()
+
+
+def _form(m, k, bits, granule, dtype, tokens, sms=148):
+    f = (ctypes.c_int64 * 10)()
+    _lib.call("gq_test_linear_form", m, k, bits, granule, dtype, tokens, sms, f)
+    return tuple(f)
+
+
+def _forms():
+    """Every form that some size reaches, by (bits, granule, dtype, columns, parts)."""
+    found = {}
+    for bits in (4, 8):
+        for granule in (32, 64, 128):
+            for dtype in (0, 1, 2):
+                for m in (16, 4096, 65536):
+                    for tokens in (1, 40, 100, 300, 5000):
+                        f = _form(m, 4096, bits, granule, dtype, tokens)
+                        if f[0]:
+                            found.setdefault((bits, granule, dtype, *f[:2]), f)
+    return found
+
+
+def test_every_form_can_be_chosen():
+    got = {(b, dt, n, parts) for b, _, dt, n, parts in _forms()}
+    want = {(b, 0, 96, parts) for b in (4, 8) for parts in (1, 2)}
+    want |= {(b, dt, n, 1) for b in (4, 8) for dt in (1, 2) for n in (64, 128)}
+    want |= {(4, dt, 128, 2) for dt in (1, 2)} | {(8, dt, 96, 2) for dt in (1, 2)}
+    assert got == want
+    assert _form(4096, 4096, 4, 128, 1, 32) == (0,) * 10 == _form(4096, 4096, 4, 128, 0, 8)
+
+
+def _early_passes(slots, barriers, runs=300, blocks=40):
+    """Two groups take the blocks of a ring in turn.  Block n is copied into slot
+    n % slots once that is free, its landing completes a phase of barrier
+    n % barriers, and a group waits for the phase's parity, so it passes where the
+    number of completed phases has another one.  Copies land, and groups look, in
+    any order.  How often a group passed before its block had landed."""
+    rng, early = random.Random(slots * 100 + barriers), 0
+    for _ in range(runs):
+        issued, landed, freed, phases = 0, set(), set(), [0] * barriers
+        at, slow = [0, 1], rng.randrange(blocks)  # the groups' blocks; one copy that takes long
+        while min(at) < blocks:
+            what = rng.randrange(4)
+            if what == 0 and issued < blocks and (issued < slots or issued - slots in freed):
+                issued += 1
+            elif what == 1:
+                flying = [n for n in range(issued) if n not in landed]
+                if flying:
+                    n = rng.choice(flying)
+                    if n != slow or len(flying) == 1 or rng.random() < 0.02:
+                        landed.add(n)
+                        phases[n % barriers] += 1
+            elif what >= 2 and at[what - 2] < blocks:
+                n = at[what - 2]
+                if phases[n % barriers] % 2 != n // barriers % 2:
+                    if n not in landed:
+                        early += 1
+                        break
+                    freed.add(n)
+                    at[what - 2] += 2
+    return early
+
+
+def test_no_group_takes_a_slot_before_its_block_has_landed():
+    assert _early_passes(3, 3) > 0  # the model sees it: a group misses every second phase
+    for key, f in _forms().items():
+        rings = [(f[4], f[5]), (f[6], f[7])] + ([(f[8], f[9])] if f[1] == 2 else [])
+        for slots, barriers in rings:
+            assert barriers % slots == 0 and _early_passes(slots, barriers, runs=30) == 0, key
+
+
+@pytest.mark.parametrize("kw", [dict(m=0), dict(k=100), dict(bits=9), dict(granule=48),
+                                dict(dtype=3), dict(tokens=0), dict(sms=0)])
+def test_form_refuses(kw):
+    a = dict(m=16, k=128, bits=4, granule=32, dtype=1, tokens=40, sms=148)
+    a.update(kw)
+    with pytest.raises(ValueError, match="gq_test_linear_form"):
+        _form(**a)
