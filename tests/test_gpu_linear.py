@@ -14,6 +14,7 @@ rounding.  float32 terms below 2^-126 (the lowest bits of numbers under
 """
 
 import copy
+import functools
 import pickle
 
 import numpy as np
@@ -22,7 +23,10 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from jax_gptq_b200 import linear, packing
+import linear_forms as F
+
+from jax_gptq_b200 import _arrays as A
+from jax_gptq_b200 import _lib, linear, packing
 from jax_gptq_b200.config import QuantConfig
 from jax_gptq_b200.gptq_ref import gptq_quantize
 from oracle import inputs
@@ -126,6 +130,38 @@ def test_many_rows(t):
     pl = linear.prepare_linear(p)
     x = _x((t, 256), torch.bfloat16, t)
     _check(linear.packed_matmul(x, pl), x, w, pl)
+
+
+@functools.lru_cache(maxsize=1)
+def _weights(m, n, group, bits):
+    """Random prepared weights with columns in order, and their float64 values."""
+    gen = torch.Generator(device="cuda").manual_seed(m + n + bits + group)
+    rand = lambda hi, *shape: torch.randint(0, hi, shape, generator=gen, device="cuda")
+    codes = rand(1 << bits, m, n).to(torch.uint8)
+    scales = (5 + 15 * torch.rand((m, n // group), generator=gen, device="cuda")) * 1e-3
+    zeros = rand(1 << bits, m, n // group).float()
+    words = _lib.lib().gq_packed_words(n, bits)
+    q = torch.empty((m, words), dtype=torch.int32, device="cuda")
+    _lib.call("gq_pack_codes", A.ptr(codes), m, n, n, bits, A.ptr(q), words, A.stream())
+    order = torch.arange(n, dtype=torch.int32, device="cuda")
+    pl = linear.prepare_linear(packing.PackedLinear(q, scales, zeros, order // group, order, bits,
+                                                    group, False, n))
+    w = (codes.double().view(m, -1, group) - zeros.double()[..., None]) * scales.double()[..., None]
+    return pl, w.view(m, n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", F.SIZES)
+@pytest.mark.parametrize("group", F.GROUPS)
+@pytest.mark.parametrize("bits", F.BITS)
+def test_every_form_of_many_tokens(bits, group, size, dtype):
+    t, m, n = size
+    pl, w = _weights(m, n, group, bits)
+    assert pl.granule == group
+    x = _x((t, n), dtype, t)
+    y = linear.packed_matmul(x, pl)
+    _check(y, x, w, pl)
+    assert torch.equal(y, linear.packed_matmul(x, pl))
 
 
 @pytest.mark.parametrize("t", [1, 12, 140])

@@ -8,6 +8,8 @@ import numpy as np
 import pytest
 import torch
 
+import linear_forms as F
+
 from jax_gptq_b200 import _lib, linear
 
 
@@ -83,12 +85,6 @@ def test_layout_refuses_before_launching(kw, text):
     assert text in _lib.lib().gq_last_error()
 
 
-def _form(m, k, bits, granule, dtype, tokens, sms=148):
-    f = (ctypes.c_int64 * 10)()
-    _lib.call("gq_test_linear_form", m, k, bits, granule, dtype, tokens, sms, f)
-    return tuple(f)
-
-
 def _forms():
     """Every form that some size reaches, by (bits, granule, dtype, columns, parts)."""
     found = {}
@@ -97,7 +93,7 @@ def _forms():
             for dtype in (0, 1, 2):
                 for m in (16, 4096, 65536):
                     for tokens in (1, 40, 100, 300, 5000):
-                        f = _form(m, 4096, bits, granule, dtype, tokens)
+                        f = F.form(m, 4096, bits, granule, dtype, tokens)
                         if f[0]:
                             found.setdefault((bits, granule, dtype, *f[:2]), f)
     return found
@@ -109,7 +105,21 @@ def test_every_form_can_be_chosen():
     want |= {(b, dt, n, 1) for b in (4, 8) for dt in (1, 2) for n in (64, 128)}
     want |= {(4, dt, 128, 2) for dt in (1, 2)} | {(8, dt, 96, 2) for dt in (1, 2)}
     assert got == want
-    assert _form(4096, 4096, 4, 128, 1, 32) == (0,) * 10 == _form(4096, 4096, 4, 128, 0, 8)
+    assert F.form(4096, 4096, 4, 128, 1, 32) == (0,) * 10 == F.form(4096, 4096, 4, 128, 0, 8)
+
+
+def test_the_sizes_of_the_gpu_tests_reach_every_form():
+    """A change of the rule that moves them off a form fails here."""
+    forms = {(bits, group, dtype, *F.form(m, n, bits, group, dtype, t)[:4])
+             for t, m, n in F.SIZES for group in F.GROUPS for bits in F.BITS for dtype in (0, 1, 2)}
+    width = lambda bits: 4 if bits <= 4 else 8
+    reached = {(width(b), g, dt, n, parts) for b, g, dt, n, parts, *_ in forms if n}
+    assert reached == {(width(b), g, dt, n, parts) for b, g, dt, n, parts in _forms()}
+    again = {(width(b), g, dt, n, parts) for b, g, dt, n, parts, split, tiles in forms
+             if split == 1 and tiles > F.SMS}
+    assert again == reached  # a CTA that goes on to another tile
+    split = {f[:5] for f in forms if f[4] == 2 and f[5] > 1}
+    assert split == {f[:5] for f in forms if f[4] == 2}
 
 
 def _early_passes(slots, barriers, runs=300, blocks=40):
@@ -158,4 +168,4 @@ def test_form_refuses(kw):
     a = dict(m=16, k=128, bits=4, granule=32, dtype=1, tokens=40, sms=148)
     a.update(kw)
     with pytest.raises(ValueError, match="gq_test_linear_form"):
-        _form(**a)
+        F.form(**a)
