@@ -157,6 +157,9 @@ int gq_set_wait_limit_ns(uint64_t ns);
  * above, *observed (device int) becomes 1, and the unit's status word reads
  * GQ_DEVERR_TIMEOUT; nothing traps or faults.  No reference counterpart. */
 int gq_test_expire_wait(int unit, int* observed, void* stream);
+/* The same for the bounded waits of the many-token packed product (one warp,
+ * two limits long). */
+int gq_test_expire_linear_wait(int* observed, void* stream);
 
 /* stats.py:4-18 for float32 activations (CUDA-core fp32 GEMM). */
 int gq_syrk_f32(const float* x, int64_t tokens, int64_t d, int64_t ldx,
@@ -412,7 +415,9 @@ int gq_unpack_dequant(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp,
  * place if it is 16-byte aligned with ldx % 8 == 0, and needs no workspace).
  * bits, granule and k as laid out.  Products are summed in float32 in a fixed
  * order and rounded once; float32 x runs as three exact bf16 terms (what lies
- * below 2^-126 may be lost).  x and y must not overlap.  workspace: 256-byte aligned,
+ * below 2^-126 may be lost).  The many-token form has bounded device-side
+ * waits: gq_check_device tells whether one expired and left y incomplete.
+ * x and y must not overlap.  workspace: 256-byte aligned,
  * gq_linear_workspace_size(tokens, k, dtype) bytes. */
 int gq_linear_layout(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp, int bits, int sym,
                      const float* scales, const float* zeros, int64_t n_groups,

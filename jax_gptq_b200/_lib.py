@@ -93,6 +93,7 @@ SIGNATURES = {
     "gq_check_device": (c_int, [_P]),
     "gq_set_wait_limit_ns": (c_int, [ctypes.c_uint64]),
     "gq_test_expire_wait": (c_int, [c_int, _P, _P]),
+    "gq_test_expire_linear_wait": (c_int, [_P, _P]),
     "gq_gptq_sweep_static": (c_int, [_P, c_int64, c_int64, c_int64, _P, _P, c_int64, _P, c_int,
                                      c_int, c_int, c_int, _P, _P, c_int, _P, _P, _P, _P, _P, _P]),
     "gq_qrcp_workspace_size": (c_int64, [c_int64, c_int64, c_int]),

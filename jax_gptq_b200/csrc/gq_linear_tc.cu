@@ -308,6 +308,30 @@ __device__ __forceinline__ void cluster_sync() {
                    : "memory");
 }
 
+// Failure-path check of this file's bounded waits: a warp waits on an mbarrier that
+// nothing arrives on, so the wait must give up after g_wait_limit_ns, record
+// GQ_DEVERR_TIMEOUT, and return false; a second wait then sees the flag, and the
+// drain, which goes on after it, ends by its own limit.  *observed gets 1 when all
+// did so.  The kernel then simply returns.
+__global__ void expire_wait_kernel(int* observed) {
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ int abort_flag;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    mbar_init(&bar, 1);
+  }
+  __syncthreads();
+  const bool first = mbar_wait_warp(&bar, 0, &abort_flag);
+  const bool second = mbar_wait_warp(&bar, 0, &abort_flag);
+  mbar_drain(&bar, 0);
+  if (threadIdx.x == 0) *observed = !first && !second && abort_flag == 1 ? 1 : 0;
+}
+
+int launch_expire_test(int* observed, cudaStream_t st) {
+  expire_wait_kernel<<<1, 32, 0, st>>>(observed);
+  return check_launch("packed product expire_wait");
+}
+
 template <int WIDTH, typename T, int N, int PARTS, int G>
 __global__ void __launch_bounds__(THREADS, 1)
 many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,

@@ -940,6 +940,7 @@ int launch_expire_test(int* observed, cudaStream_t st);
 namespace lintc {
 int read_status(int reset, int* out);
 int set_wait_limit(uint64_t ns);
+int launch_expire_test(int* observed, cudaStream_t st);
 }
 
 }  // namespace gq
@@ -979,6 +980,11 @@ int gq_test_expire_wait(int unit, int* observed, void* stream) {
   if (unit == 1) return gq::tc32::launch_expire_test(observed, gq::as_stream(stream));
   gq::tc::expire_wait_kernel<<<1, 32, 0, gq::as_stream(stream)>>>(observed);
   return gq::check_launch("bf16 expire_wait");
+}
+
+int gq_test_expire_linear_wait(int* observed, void* stream) {
+  GQ_REQUIRE(observed != nullptr, "gq_test_expire_linear_wait: NULL observed");
+  return gq::lintc::launch_expire_test(observed, gq::as_stream(stream));
 }
 
 int gq_check_device(void* stream) {

@@ -47,7 +47,8 @@ def masked_nll_from_logits(logits, labels) -> tuple[float, int]:
 
 
 def evaluate_perplexity(model: Callable, windows: List, labels: List, batch_size: int = 1) -> float:
-    """eval.py:25-48 for ``model(input_ids) -> logits [B, T, V]``."""
+    """eval.py:25-48 for ``model(input_ids) -> logits [B, T, V]``.  Raises
+    ``_lib.DeviceTimeout`` where a kernel's bounded wait expired on the way."""
     total_nll, total_tokens = 0.0, 0
     for i in range(0, len(windows), batch_size):
         end = min(i + batch_size, len(windows))
@@ -58,6 +59,8 @@ def evaluate_perplexity(model: Callable, windows: List, labels: List, batch_size
         nll, tokens = masked_nll_from_logits(logits, label_batch)
         total_nll += nll
         total_tokens += tokens
+    if len(windows):
+        _lib.check_device()  # a bounded wait that expired left incomplete logits
     if total_tokens == 0:
         return float("nan")
     return float(np.exp(total_nll / total_tokens))

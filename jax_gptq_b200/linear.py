@@ -134,7 +134,12 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     it loses no bits above 2^-126) and rounded once.  numpy in -> numpy out.
     ``out``, if given, is a contiguous tensor of the result's shape and type
     that does not share memory with ``x``.  There is no gradient: an ``x`` that
-    asks for one is refused."""
+    asks for one is refused.
+
+    Waits inside the kernel are bounded.  One that expired leaves the result
+    incomplete and a status word behind, which this call does not read (it
+    would have to wait for the device): ``_lib.check_device()`` raises on it,
+    and ``TinyLM.generate`` and ``evaluate_perplexity`` call that at their end."""
     dt = _DTYPES.get(getattr(x, "dtype", None))
     if dt is None:
         if A.is_host(x):

@@ -38,7 +38,7 @@ from dataclasses import dataclass, field
 import torch
 import torch.nn.functional as F
 
-from . import linear, packing, rotary, sampling, stats
+from . import _lib, linear, packing, rotary, sampling, stats
 from .config import QuantConfig
 from .gptq_ref import SweepResult, factor_hessian, gptq_sweep
 from .qronos_ref import qronos_quantize
@@ -342,7 +342,9 @@ class TinyLM(torch.nn.Module):
         """Continue the prompts ``ids`` [B, T] by one token per column of the
         uniform numbers ``u`` [B, new], chosen as ``sampling.sample_tokens``
         does; returns tokens and log-probabilities [B, new].  A row that is
-        left without a token (NaN logits) goes on from token 0."""
+        left without a token (NaN logits) goes on from token 0.  Waits for the
+        device at the end, and raises ``_lib.DeviceTimeout`` where a kernel's
+        bounded wait expired on the way."""
         if ids.dim() != 2 or ids.shape[1] < 1 or u.dim() != 2 or u.shape[0] != ids.shape[0]:
             raise ValueError(f"ids must be [B, T >= 1] and u [B, new], got {tuple(ids.shape)} and "
                              f"{tuple(u.shape)}")
@@ -361,6 +363,8 @@ class TinyLM(torch.nn.Module):
             got = sampling.sample_tokens(logits, u[:, i], temperature, top_k, top_p, min_p)
             tokens[:, i], logprobs[:, i] = got
             ids = got.tokens.clamp_min(0)[:, None]
+        if new:
+            _lib.check_device()  # a bounded wait that expired left incomplete logits
         return sampling.Sampled(tokens, logprobs)
 
 

@@ -74,3 +74,41 @@ def test_wait_limit_range_is_checked():
         _lib.call("gq_set_wait_limit_ns", 10)
     with pytest.raises(ValueError, match="outside"):
         _lib.call("gq_set_wait_limit_ns", 10 ** 12)
+
+
+def _expire():
+    """A wait of the many-token packed product that nothing satisfies."""
+    obs = torch.full((1,), -1, dtype=torch.int32, device="cuda")
+    _lib.call("gq_test_expire_linear_wait", A.ptr(obs), A.stream())
+    return obs
+
+
+def test_expired_wait_of_the_packed_product(short_wait_limit):
+    t0 = time.perf_counter()
+    obs = _expire()
+    with pytest.raises(_lib.DeviceTimeout, match="bounded device-side wait expired"):
+        _lib.check_device()
+    elapsed = time.perf_counter() - t0
+    assert obs.item() == 1
+    assert short_wait_limit <= elapsed < 1.5, elapsed
+    _lib.check_device()  # the word was cleared by the check
+
+
+def test_generate_and_perplexity_tell_of_expired_waits(short_wait_limit):
+    """A wait that expires in one of a model's products: no tokens and no
+    perplexity, but an error, and the next run is as before."""
+    from jax_gptq_b200 import eval as E
+    from jax_gptq_b200 import pipeline
+    cfg = pipeline.BlockConfig(hidden=128, intermediate=256, heads=2, kv_heads=1)
+    lm = pipeline.TinyLM(pipeline.synth_stack(1, cfg), 50, cfg)
+    ids, u = torch.ones((1, 4), dtype=torch.int64, device="cuda"), torch.rand((1, 2), device="cuda")
+    windows = [ids.cpu().numpy()]
+    want, score = lm.generate(ids, u), E.evaluate_perplexity(lm, windows, windows)
+    handle = lm.blocks[0].down_proj.register_forward_hook(lambda *_: (_expire(), None)[1])
+    with pytest.raises(_lib.DeviceTimeout):
+        lm.generate(ids, u)
+    with pytest.raises(_lib.DeviceTimeout):
+        E.evaluate_perplexity(lm, windows, windows)
+    handle.remove()
+    assert torch.equal(lm.generate(ids, u).tokens, want.tokens)
+    assert E.evaluate_perplexity(lm, windows, windows) == score
