@@ -65,8 +65,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
         raise ValueError(f"logits must be on a CUDA device, got {logits.device}")
     lg = logits if logits.dim() == 2 else logits[None]
     rows, vocab = lg.shape
-    if lg.stride(1) != 1 or lg.stride(0) < vocab:
+    if lg.stride(1) != 1 or (rows > 1 and lg.stride(0) < vocab):
         lg = lg.contiguous()
+    ld = lg.stride(0) if rows > 1 else vocab  # (one row's stride may be any number)
     if u.dtype not in (torch.float32, torch.float64):
         raise ValueError(f"u must be float32 or float64, got {u.dtype}")
     dev = lg.get_device()
@@ -84,7 +85,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     tokens = torch.empty_like(u, dtype=torch.int64)
     logprobs = torch.empty_like(u, dtype=torch.float32)
     if rows:
-        status = _lib.lib().gq_sample(lg.data_ptr(), dt, rows, vocab, lg.stride(0), up, uk, tp, tk,
+        status = _lib.lib().gq_sample(lg.data_ptr(), dt, rows, vocab, ld, up, uk, tp, tk,
                                       tv, kp, kk, kv, pp, pk, pv, mp, mk, mv, tokens.data_ptr(),
                                       logprobs.data_ptr(), A.raw_stream(dev))
         if status:

@@ -112,6 +112,21 @@ def test_odd_vocabularies_and_strides(vocab):
     assert one.tokens.shape == (1,)
 
 
+def test_one_row_of_any_row_stride():
+    """The stride of a dimension of one element says nothing."""
+    z, u = _logits(1, 5000, torch.float32, 21)
+    want = sampling.sample_tokens(z, u, top_k=40, top_p=0.9)
+    column = z.t().contiguous()  # [vocab, 1]
+    for row in (column.t(), z[0].as_strided((1, 5000), (1, 1)), z[0].as_strided((1, 5000), (0, 1)),
+                z[0].as_strided((1, 5000), (77777, 1)), z[0].expand(1, 5000)):
+        assert row.shape == (1, 5000)
+        for uu in (u, u[0], u.as_strided((1,), (9,))):
+            got = sampling.sample_tokens(row, uu, top_k=40, top_p=0.9)
+            assert torch.equal(got.tokens, want.tokens) and torch.equal(got.logprobs, want.logprobs)
+    one = sampling.sample_tokens(z[:, :1].as_strided((1, 1), (3, 5)), u)
+    assert one.tokens.tolist() == [0] and one.logprobs.tolist() == [0.0]
+
+
 @pytest.mark.parametrize("rows", [1, 2, 40, 75, 149, 300, 1000])
 def test_many_rows(rows):
     z, u = _logits(rows, 9001, torch.float32, rows)
