@@ -149,6 +149,13 @@ def _heads(name: str, x: torch.Tensor, plan: RotaryPlan) -> torch.Tensor:
     return x if x.stride(3) == 1 else x.contiguous()
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A new tensor of x's layout; contiguous where that of an overlapping x would
+    not leave the components so."""
+    o = torch.empty_like(x)
+    return o if o.stride(3) == 1 else x.new_empty(x.shape)
+
+
 def _results(q, k, out):
     oq, ok = out
     if oq is None or (ok is None) != (k is None):
@@ -227,7 +234,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if not positions.is_contiguous() and positions.stride(-1) != 1:
         positions = positions.contiguous()
     if out is None:
-        oq, ok = torch.empty_like(q), None if k is None else torch.empty_like(k)
+        oq, ok = _like(q), None if k is None else _like(k)
     else:
         oq, ok = _results(q, k, out)
     if b == 0 or s == 0 or h + hk == 0:

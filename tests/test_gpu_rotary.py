@@ -129,6 +129,27 @@ def test_layouts_alignment_and_in_place(interleaved, dtype):
     _check(rotary.apply_rotary(x, None, pos[:, ::1].t().contiguous().t(), plan)[0], x, pos, plan, inv)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_overlapping_inputs(interleaved, dtype):
+    """Views whose elements share memory: the result has memory of its own, with
+    contiguous components, whatever the order of the view's strides."""
+    plan = rotary.rotary_plan(8, rotary_dim=6, interleaved=interleaved)
+    inv, _ = rotary.rotary_frequencies(6)
+    x = torch.randn((2, 3, 12), device="cuda").to(dtype)
+    pos = torch.randint(0, 3000, (2, 5), device="cuda")
+    for v in (x.unfold(2, 8, 1), x.unfold(2, 8, 1)[:, :2, :2],
+              x.as_strided((2, 3, 5, 8), (1, 1, 1, 1)), x.as_strided((2, 3, 5, 8), (0, 0, 0, 1))):
+        p = pos[:, :v.shape[2]]
+        oq, ok = rotary.apply_rotary(v, v, p, plan)
+        assert oq.stride(3) == 1 and ok.stride(3) == 1
+        _check(oq, v, p, plan, inv)
+        assert torch.equal(oq, ok)
+        g = v.clone().requires_grad_()
+        gx, = torch.autograd.grad(rotary.apply_rotary(g, None, p, plan)[0], g, v)
+        _check(gx, v, p, plan, inv, transpose=True)
+
+
 def test_gradient_is_the_transposed_map():
     plan = rotary.rotary_plan(16, rotary_dim=12, scaling=rotary.YarnScaling(4.0, 64))
     inv, _ = rotary.rotary_frequencies(12, scaling=rotary.YarnScaling(4.0, 64))
