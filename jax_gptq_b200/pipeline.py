@@ -163,8 +163,11 @@ def attach_packed(blocks: list[DecoderBlock], checkpoint_dir: str) -> None:
     """Replace the linears of ``blocks`` by :class:`linear.QuantLinear` on the
     packed weights of ``checkpoint_dir`` (the ``layer{i}.pt`` files that
     :func:`quantize_stack` wrote).  The blocks then run, but can no longer be
-    quantized: their float weights are gone."""
-    for i, blk in enumerate(blocks):
+    quantized: their float weights are gone.  Every file is read and laid out once
+    before the first linear is replaced, so that a missing or bad one leaves all
+    blocks as they were (laying all out before would need room for both forms)."""
+
+    def laid_out(i, blk):
         path = os.path.join(checkpoint_dir, f"layer{i}.pt")
         packed = packing.load_layer(path, device="cuda")
         if set(packed) != set(GROUPS):
@@ -174,8 +177,17 @@ def attach_packed(blocks: list[DecoderBlock], checkpoint_dir: str) -> None:
             if (p.m, p.n) != (lin.out_features, lin.in_features):
                 raise ValueError(f"{path}: {name} is {p.m} x {p.n}, the block's is "
                                  f"{lin.out_features} x {lin.in_features}")
-        for name, p in packed.items():
-            setattr(blk, name, linear.QuantLinear(p))
+            try:
+                yield name, linear.QuantLinear(p)
+            except ValueError as e:
+                raise ValueError(f"{path}: {name}: {e}") from e
+
+    for i, blk in enumerate(blocks):
+        for _ in laid_out(i, blk):
+            pass
+    for i, blk in enumerate(blocks):
+        for name, lin in laid_out(i, blk):
+            setattr(blk, name, lin)
 
 
 def synth_stack(n_layers: int, cfg: BlockConfig, seed: int = 0, std: float = 0.02,

@@ -119,3 +119,28 @@ def test_refusals(models, tmp_path):
     with pytest.raises(ValueError, match="4 positions"):
         blk.decode(torch.zeros((1, 5, 256), dtype=torch.bfloat16, device="cuda"), cache,
                    rotary.rotary_plan(64))
+
+
+def test_a_bad_file_leaves_every_block_as_it_was(models, tmp_path):
+    import shutil
+
+    from jax_gptq_b200 import packing
+    path = models[2]
+    blocks = pipeline.synth_stack(2, CFG)
+    before = [{n: getattr(b, n) for n in pipeline.GROUPS} for b in blocks]
+    good = packing.load_layer(f"{path}/layer1.pt")
+    last = list(pipeline.GROUPS)[-1]
+    scales = good[last].scales.clone()
+    scales[0, 0] = float("nan")
+    bad = [None, {n: good[n] for n in list(pipeline.GROUPS)[:-1]},
+           {**good, last: packing.PackedLinear(**{**good[last].__dict__, "scales": scales})}]
+    for layer, error in zip(bad, ((FileNotFoundError, "layer1"), (ValueError, "a block has"),
+                                  (ValueError, f"layer1.pt: {last}: scales must be finite"))):
+        shutil.copy(f"{path}/layer0.pt", tmp_path / "layer0.pt")
+        if layer is not None:
+            packing.save_layer(str(tmp_path / "layer1.pt"), layer)
+        with pytest.raises(error[0], match=error[1]):
+            pipeline.attach_packed(blocks, str(tmp_path))
+        assert all(getattr(b, n) is lin for b, kept in zip(blocks, before) for n, lin in kept.items())
+    pipeline.attach_packed(blocks, path)
+    assert all(isinstance(getattr(b, n), linear.QuantLinear) for b in blocks for n in pipeline.GROUPS)
