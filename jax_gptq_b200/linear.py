@@ -82,6 +82,12 @@ def _positions(g_idx: torch.Tensor, n_groups: int):
     return granule, k, kmap, gg
 
 
+def _on_current(p: PackedLinear):
+    """(qweight, g_idx, scales, zeros) on the current device, wherever they are."""
+    s, z = (A.to_device(t.cuda()) for t in (p.scales, p.zeros))
+    return p.qweight.cuda().contiguous(), p.g_idx.cuda(), s, z
+
+
 def prepare_linear(p: PackedLinear) -> PreparedLinear:
     """Lay ``p`` out for ``packed_matmul`` on the current device (once per weight).
 
@@ -104,8 +110,7 @@ def prepare_linear(p: PackedLinear) -> PreparedLinear:
                          f"{tuple(p.scales.shape)} and {tuple(p.zeros.shape)}")
     if tuple(p.g_idx.shape) != (n,):
         raise ValueError(f"g_idx must be [{n}], got {tuple(p.g_idx.shape)}")
-    q, g_idx = p.qweight.cuda().contiguous(), p.g_idx.cuda()
-    s, z = A.to_device(p.scales), A.to_device(p.zeros)
+    q, g_idx, s, z = _on_current(p)
     lo, hi = (int(v) for v in torch.aminmax(g_idx))
     if lo < 0 or hi >= s.shape[1]:
         raise ValueError(f"g_idx must lie in [0, {s.shape[1]}), got {lo} .. {hi}")

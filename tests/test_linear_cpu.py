@@ -10,7 +10,7 @@ import torch
 
 import linear_forms as F
 
-from jax_gptq_b200 import _lib, linear
+from jax_gptq_b200 import _lib, linear, packing
 
 
 @pytest.mark.parametrize("counts,granule,k", [([128, 128], 128, 256), ([64, 64, 64], 64, 256),
@@ -169,3 +169,24 @@ def test_form_refuses(kw):
     a.update(kw)
     with pytest.raises(ValueError, match="gq_test_linear_form"):
         F.form(**a)
+
+
+def test_weights_of_another_device_are_moved(monkeypatch):
+    """prepare_linear hands addresses of the current device alone to its launch."""
+    class Here(torch.Tensor):
+        is_cuda = True
+
+    class There(torch.Tensor):  # of another device: cuda() copies it to the current one
+        is_cuda = True
+
+        def cuda(self):
+            return self.clone().as_subclass(Here)
+
+    monkeypatch.setattr(linear.A, "require_cuda", lambda: None)
+    there = lambda *shape, dtype=torch.float32: torch.ones(shape, dtype=dtype).as_subclass(There)
+    p = packing.PackedLinear(there(4, 8, dtype=torch.int32), there(4, 2), there(4, 2),
+                             there(64, dtype=torch.int32), there(64, dtype=torch.int32), 4, 32,
+                             False, 64)
+    moved = linear._on_current(p)
+    assert all(type(t) is Here for t in moved)
+    assert [tuple(t.shape) for t in moved] == [(4, 8), (64,), (4, 2), (4, 2)]
