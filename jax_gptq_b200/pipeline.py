@@ -169,7 +169,7 @@ def attach_packed(blocks: list[DecoderBlock], checkpoint_dir: str) -> None:
 
     def laid_out(i, blk):
         path = os.path.join(checkpoint_dir, f"layer{i}.pt")
-        packed = packing.load_layer(path, device="cuda")
+        packed = packing.load_layer(path)
         if set(packed) != set(GROUPS):
             raise ValueError(f"{path} holds {sorted(packed)}, a block has {sorted(GROUPS)}")
         for name, p in packed.items():
@@ -178,9 +178,11 @@ def attach_packed(blocks: list[DecoderBlock], checkpoint_dir: str) -> None:
                 raise ValueError(f"{path}: {name} is {p.m} x {p.n}, the block's is "
                                  f"{lin.out_features} x {lin.in_features}")
             try:
-                yield name, linear.QuantLinear(p)
+                with torch.cuda.device_of(blk.input_layernorm.weight):  # the block's device
+                    lin = linear.QuantLinear(p)
             except ValueError as e:
                 raise ValueError(f"{path}: {name}: {e}") from e
+            yield name, lin
 
     for i, blk in enumerate(blocks):
         for _ in laid_out(i, blk):
@@ -360,19 +362,23 @@ class TinyLM(torch.nn.Module):
         if ids.dim() != 2 or ids.shape[1] < 1 or u.dim() != 2 or u.shape[0] != ids.shape[0]:
             raise ValueError(f"ids must be [B, T >= 1] and u [B, new], got {tuple(ids.shape)} and "
                              f"{tuple(u.shape)}")
+        with torch.cuda.device_of(ids):  # the model's device, which may not be the current one
+            return self._generate(ids, u, temperature, top_k, top_p, min_p)
+
+    def _generate(self, ids, u, *settings) -> sampling.Sampled:
         cfg = self.blocks[0].cfg
         plan = rotary.rotary_plan(cfg.hidden // cfg.heads, theta=cfg.rope_theta)
-        new = u.shape[1]
+        b, new, dev = ids.shape[0], u.shape[1], ids.device
         dtype = self.embed.weight.dtype
-        caches = [KVCache.empty(cfg, ids.shape[0], ids.shape[1] + new, dtype) for _ in self.blocks]
-        tokens = torch.empty((ids.shape[0], new), dtype=torch.int64, device=ids.device)
-        logprobs = torch.empty((ids.shape[0], new), dtype=torch.float32, device=ids.device)
+        caches = [KVCache.empty(cfg, b, ids.shape[1] + new, dtype, dev) for _ in self.blocks]
+        tokens = torch.empty((b, new), dtype=torch.int64, device=dev)
+        logprobs = torch.empty((b, new), dtype=torch.float32, device=dev)
         for i in range(new):
             x = self.embed(ids)
             for blk, cache in zip(self.blocks, caches):
                 x = blk.decode(x, cache, plan)
             logits = self.lm_head(self.norm(x[:, -1]))
-            got = sampling.sample_tokens(logits, u[:, i], temperature, top_k, top_p, min_p)
+            got = sampling.sample_tokens(logits, u[:, i], *settings)
             tokens[:, i], logprobs[:, i] = got
             ids = got.tokens.clamp_min(0)[:, None]
         if new:
