@@ -148,6 +148,8 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     dt = _DTYPES.get(getattr(x, "dtype", None))
     if dt is None:
         if A.is_host(x):
+            if out is not None:
+                raise ValueError("out goes with a tensor x, not with a host array")
             return A.like_input(packed_matmul(A.to_device(x), w), x)
         raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
     if x.requires_grad and torch.is_grad_enabled():

@@ -190,3 +190,8 @@ def test_weights_of_another_device_are_moved(monkeypatch):
     moved = linear._on_current(p)
     assert all(type(t) is Here for t in moved)
     assert [tuple(t.shape) for t in moved] == [(4, 8), (64,), (4, 2), (4, 2)]
+
+
+def test_out_with_a_host_array_is_refused():
+    with pytest.raises(ValueError, match="host array"):
+        linear.packed_matmul(np.zeros((2, 64), np.float32), None, out=torch.zeros(2, 4))
