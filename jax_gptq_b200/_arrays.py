@@ -109,6 +109,13 @@ def _apart(a, b, da, db, common) -> bool:
     return True
 
 
+def written(*tensors) -> None:
+    """Tells autograd that a kernel writes the caller's tensors: a graph that kept
+    one of them for its backward pass then raises, as after torch's own in-place
+    operations."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
 def distinct_elements(t: torch.Tensor) -> bool:
     """Whether no two elements of ``t`` share memory, judged by its strides:
     each is at least the span of the ones below it."""

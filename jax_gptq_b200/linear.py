@@ -166,7 +166,8 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) < n:
         x2 = x.reshape(-1, n).contiguous()
     tokens, ldx = x2.shape[0], x2.stride(0)
-    if out is None:
+    given = out is not None
+    if not given:
         out = x.new_empty(tokens, m) if x2 is x else x.new_empty(*x.shape[:-1], m)
     elif tuple(out.shape) != (*x.shape[:-1], m) or out.dtype != x.dtype or \
             out.device != x.device or not out.is_contiguous():
@@ -176,6 +177,8 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
         raise ValueError("out shares memory with x")
     if tokens == 0 or m == 0:
         return out
+    if given:
+        A.written(out)
     lib = _lib.lib()
     xp, wp, nbytes = x2.data_ptr(), None, 0
     if not (w.direct and dt and xp % 16 == 0 and ldx % 8 == 0):  # x is first put in order

@@ -237,6 +237,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         oq, ok = _like(q), None if k is None else _like(k)
     else:
         oq, ok = _results(q, k, out)
+        A.written(oq, ok)
     if b == 0 or s == 0 or h + hk == 0:
         return oq, ok
     q0, q1, q2, _ = q.stride()

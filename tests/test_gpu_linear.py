@@ -332,3 +332,18 @@ def test_gradients_are_refused():
     with torch.no_grad():
         want = lin(x)
     assert torch.equal(lin(x.detach()), want)
+
+
+def test_autograd_sees_that_out_is_written():
+    """A tensor that a graph keeps for its backward pass, written in between."""
+    p, _ = _packed(64, 64, 32, 4, False, 8, act_order=False)
+    pl = linear.prepare_linear(p)
+    leaf = _x((5, 64), torch.float32, 1).requires_grad_()
+    y = leaf.exp()  # kept: its gradient is itself
+    with torch.no_grad():
+        linear.packed_matmul(_x((5, 64), torch.float32, 2), pl, out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():  # (tensors without a version)
+        out = torch.empty((5, 64), device="cuda")
+        assert linear.packed_matmul(_x((5, 64), torch.float32, 2), pl, out=out) is out

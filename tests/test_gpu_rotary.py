@@ -249,3 +249,19 @@ def test_gradients(kv_heads, interleaved, dtype):
     _check(gq, torch.ones_like(q), pos, plan, inv, transpose=True)
     with pytest.raises(ValueError, match="out takes no gradients"):
         rotary.apply_rotary(q, None, pos, plan, out=(torch.empty_like(q), None))
+
+
+def test_autograd_sees_what_is_turned_in_place():
+    """Tensors that a graph keeps for its backward pass, turned in between."""
+    plan = rotary.rotary_plan(64)
+    pos = torch.arange(9, device="cuda")
+    for pair in ((True, False), (True, True)):
+        leaf = _heads(2, 4, 9, 64, torch.float32, 1).requires_grad_()
+        q, k = leaf.exp(), leaf.exp() if pair[1] else None  # kept: their gradient is themselves
+        with torch.no_grad():
+            rotary.apply_rotary(q, k, pos, plan, out=(q, k))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            (k if pair[1] else q).sum().backward()
+    with torch.inference_mode():  # (tensors without a version)
+        q = _heads(2, 4, 9, 64, torch.float32, 1)
+        assert rotary.apply_rotary(q, None, pos, plan, out=(q, None))[0] is q
