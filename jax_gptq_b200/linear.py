@@ -138,7 +138,8 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     Products are summed in float32 (float32 x runs as three exact bf16 terms:
     it loses no bits above 2^-126) and rounded once.  numpy in -> numpy out.
     ``out``, if given, is a contiguous tensor of the result's shape and type
-    that does not share memory with ``x``.  There is no gradient: an ``x`` that
+    that does not share memory with ``x`` (under ``torch.no_grad()`` where it asks
+    for gradients).  There is no gradient: an ``x`` that
     asks for one is refused.
 
     Waits inside the kernel are bounded.  One that expired leaves the result
@@ -175,6 +176,8 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
                          f"{x.device}")
     elif A.overlap(out, x2):
         raise ValueError("out shares memory with x")
+    elif out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out takes no gradients: call it under torch.no_grad()")
     if tokens == 0 or m == 0:
         return out
     if given:

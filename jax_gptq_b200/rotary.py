@@ -160,6 +160,8 @@ def _results(q, k, out):
     oq, ok = out
     if oq is None or (ok is None) != (k is None):
         raise ValueError("out must be a pair like (q, k)")
+    if torch.is_grad_enabled() and (oq.requires_grad or (ok is not None and ok.requires_grad)):
+        raise ValueError("out takes no gradients: call it under torch.no_grad()")
     pairs = [("q", q, oq)] + ([] if k is None else [("k", k, ok)])
     for name, x, o in pairs:
         if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device or \

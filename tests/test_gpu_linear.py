@@ -347,3 +347,15 @@ def test_autograd_sees_that_out_is_written():
     with torch.inference_mode():  # (tensors without a version)
         out = torch.empty((5, 64), device="cuda")
         assert linear.packed_matmul(_x((5, 64), torch.float32, 2), pl, out=out) is out
+
+
+def test_out_that_asks_for_gradients_is_refused():
+    p, _ = _packed(64, 64, 32, 4, False, 8, act_order=False)
+    pl = linear.prepare_linear(p)
+    x = _x((5, 64), torch.float32, 1)
+    leaf = torch.zeros((5, 64), device="cuda", requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(ValueError, match="out takes no gradients"):
+            linear.packed_matmul(x, pl, out=out)
+        with torch.no_grad():
+            assert torch.equal(linear.packed_matmul(x, pl, out=out), linear.packed_matmul(x, pl))

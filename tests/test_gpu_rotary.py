@@ -265,3 +265,17 @@ def test_autograd_sees_what_is_turned_in_place():
     with torch.inference_mode():  # (tensors without a version)
         q = _heads(2, 4, 9, 64, torch.float32, 1)
         assert rotary.apply_rotary(q, None, pos, plan, out=(q, None))[0] is q
+
+
+def test_out_that_asks_for_gradients_is_refused():
+    plan = rotary.rotary_plan(64)
+    pos = torch.arange(9, device="cuda")
+    q = _heads(2, 4, 9, 64, torch.float32, 1)
+    leaf = torch.zeros_like(q, requires_grad=True)
+    plain = torch.zeros_like(q)
+    for k, out in ((None, (leaf, None)), (q, (plain, leaf)), (q, (plain, leaf * 2))):
+        with pytest.raises(ValueError, match="out takes no gradients"):
+            rotary.apply_rotary(q, k, pos, plan, out=out)
+        with torch.no_grad():
+            got = rotary.apply_rotary(q, k, pos, plan, out=out)
+        assert torch.equal(got[0], rotary.apply_rotary(q, None, pos, plan)[0])
