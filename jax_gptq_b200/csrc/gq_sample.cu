@@ -8,8 +8,8 @@
 //   less than p of their mass lies; min-p, of those, the ones with e_i >= min_p;
 //   the first always stays.  W = sum of e over the kept tokens;
 //   token = the smallest index i with  sum of kept e_j, j <= i  >  u W.
-// Temperature 0 (or below, or NaN) is the first largest logit.  A row without
-// any token gives -1 and -inf.
+// Temperature 0 (or below, or NaN) is the first largest logit, one above 0 but below
+// 1e-37 counts as 1e-37.  A row without any token gives -1 and -inf.
 //
 // Sums.  The choice turns on sums that lie next to a border, so e is computed
 // in float64 and held as a whole number of 2^-S (S = 45 for up to 2^17 tokens):
@@ -475,13 +475,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   rw.mx = (double)mx;
   rw.top = mx;
   rw.roots = &sh.roots;
-  rw.c = fmin(1.4426950408889634 / temp, 1e300);
+  rw.c = 1.4426950408889634 / fmax(temp, 1e-37);  // bins are found in float32: 11 c has to be one
   rw.scale = a.scale;
   rw.limit = (double)(((__double2hiint(a.scale) >> 20) & 0x7ff) - 1023) + 2.0;  // S + 2
   rw.low = __double2float_rd(rw.mx - 60.0 / rw.c);
   const double low_y = (rw.mx - (double)rw.low) * rw.c;  // 0 where the largest is huge, NaN where infinite
   rw.plain = rw.low > -INFINITY && low_y > 59.0 && low_y < 1000.0;
-  const float cf = (float)fmin(rw.c, 3e38);
+  const float cf = (float)rw.c;
   // bin of a token; the last bin holds only terms that are zero (46.45 powers of
   // two below the largest and further), and whatever is no token at all
   auto depth = [&](float l) {  // in bins

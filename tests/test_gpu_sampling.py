@@ -228,6 +228,21 @@ def test_top_k_with_min_p_on_coarse_logits(k):
     _check(z.float(), u, temperature=t, top_k=k, min_p=mp)
 
 
+def test_lowest_temperatures():
+    """Logits that differ by subnormal numbers, at temperatures of their size: one
+    below 1e-37 counts as 1e-37."""
+    z = torch.zeros((4, 3000), device="cuda")
+    z += torch.arange(3000, device="cuda") % 50 * -4e-39
+    u = torch.tensor([0.0, 0.3, 0.6, 0.999], device="cuda")
+    for setting in (dict(top_k=2), dict(top_k=200), dict(top_p=0.3), dict(min_p=0.9),
+                    dict(top_k=500, top_p=0.9, min_p=0.8), dict()):
+        want = _check(z, u, temperature=1e-37, **setting)
+        for t in (2e-38, 1e-40, 1e-300):
+            got = sampling.sample_tokens(z, u, temperature=t, **setting)
+            assert torch.equal(got.tokens, want.tokens) and torch.equal(got.logprobs, want.logprobs)
+        _check(z * 100, u, temperature=1e-36, **setting)
+
+
 def test_settings_per_row():
     rows = 64
     z, u = _logits(rows, 20011, torch.float32, 5)
