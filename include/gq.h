@@ -467,8 +467,8 @@ int gq_rotary(const void* q, void* q_out, int64_t heads, const void* k, void* k_
  * tokens[row] = the smallest index i for which the sum of e over kept tokens
  * 0 .. i exceeds u times the sum over all kept (u of 1 or more: the last kept);
  * logprobs[row] (or NULL) = log of its share of the kept mass.  temperature
- * not above 0: the first largest logit, logprob 0; above 0 it is at least
- * 1e-37.  A row without a token: -1
+ * not above 0: the first largest logit, logprob 0; others count as at
+ * least 1e-37 and at most 1e36.  A row without a token: -1
  * and -inf.  Sums are of whole numbers of 2^-45 (2^-42 for the largest
  * vocabularies) of the largest term, independent of any order. */
 int gq_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,

@@ -8,8 +8,8 @@
 //   less than p of their mass lies; min-p, of those, the ones with e_i >= min_p;
 //   the first always stays.  W = sum of e over the kept tokens;
 //   token = the smallest index i with  sum of kept e_j, j <= i  >  u W.
-// Temperature 0 (or below, or NaN) is the first largest logit, one above 0 but below
-// 1e-37 counts as 1e-37.  A row without any token gives -1 and -inf.
+// Temperature 0 (or below, or NaN) is the first largest logit; others count as at least
+// 1e-37 and at most 1e36.  A row without any token gives -1 and -inf.
 //
 // Sums.  The choice turns on sums that lie next to a border, so e is computed
 // in float64 and held as a whole number of 2^-S (S = 45 for up to 2^17 tokens):
@@ -475,7 +475,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   rw.mx = (double)mx;
   rw.top = mx;
   rw.roots = &sh.roots;
-  rw.c = 1.4426950408889634 / fmax(temp, 1e-37);  // bins are found in float32: 11 c has to be one
+  // bins are found in float32: 11 c has to be one, and where mx - l is infinite, between
+  // numbers of opposite sign, the term has to be zero
+  rw.c = 1.4426950408889634 / fmin(fmax(temp, 1e-37), 1e36);
   rw.scale = a.scale;
   rw.limit = (double)(((__double2hiint(a.scale) >> 20) & 0x7ff) - 1023) + 2.0;  // S + 2
   rw.low = __double2float_rd(rw.mx - 60.0 / rw.c);

@@ -52,8 +52,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     that share of their mass lies; ``min_p`` keeps of those the ones with
     e >= min_p.  The most likely token always stays.  The result is the
     smallest index at which the running sum of the kept e exceeds u times their
-    total.  ``temperature`` 0 takes the first largest logit, above 0 it is at
-    least 1e-37.  NaN and -inf
+    total.  ``temperature`` 0 takes the first largest logit; others count as
+    at least 1e-37 and at most 1e36.  NaN and -inf
     logits are never taken; a row with nothing else gives -1 and -inf.  The
     results carry no gradients."""
     dt = _DTYPES.get(logits.dtype)

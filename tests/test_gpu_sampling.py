@@ -243,6 +243,24 @@ def test_lowest_temperatures():
         _check(z * 100, u, temperature=1e-36, **setting)
 
 
+def test_highest_temperatures():
+    """Logits further apart than the largest float32: a temperature above 1e36 counts
+    as 1e36, where such a term is zero for every way of finding it."""
+    z = torch.full((4, 3000), -3.2e38, device="cuda")
+    z[:, ::2] = 3.3e38
+    z[:, ::7] = 3.1e38
+    z[:, ::11] = 3e36
+    u = torch.tensor([0.0, 0.3, 0.6, 0.999], device="cuda")
+    for setting in (dict(), dict(top_k=2), dict(top_k=1400), dict(top_k=2500), dict(top_p=0.99),
+                    dict(min_p=1e-9), dict(top_k=2900, top_p=0.9999, min_p=1e-14)):
+        want = _check(z, u, temperature=1e36, **setting)
+        for t in (1e38, 1e300, INF):
+            got = sampling.sample_tokens(z, u, temperature=t, **setting)
+            assert torch.equal(got.tokens, want.tokens) and torch.equal(got.logprobs, want.logprobs)
+    flat = _logits(4, 3000, torch.float32, 3)[0]
+    _check(flat, u, temperature=1e36, top_p=0.5)
+
+
 def test_settings_per_row():
     rows = 64
     z, u = _logits(rows, 20011, torch.float32, 5)
