@@ -8,8 +8,10 @@
 // Angles.  w_i comes as a whole number of 2^-64 turns, so p * w_i modulo one
 // turn is a 64-bit integer product that wraps: no digit of the angle is lost
 // at far positions (or negative ones), where a float32 angle at position 10^6
-// is off by 0.06.  The wrapped product, a signed fraction of half a turn,
-// becomes a float32 argument of sincospif.
+// is off by 0.06.  What the wrapped product lies from the nearest quarter turn
+// is the argument of sincospif, so that its rounding to float32 is relative to
+// at most an eighth of a turn, and cosines and sines next to 0 keep their digits
+// (of the signed half turn it would be up to 9e-8 of any of them).
 //
 // Bound: HBM (or, for a few tokens, the launch).  Each block takes some
 // positions of one batch entry, works out their cosines and sines once for all
@@ -152,11 +154,19 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(Args a) {
     const int64_t pi = b * a.pos_b + s0 + tok;
     const int64_t pos = a.pos32 ? (int64_t)static_cast<const int32_t*>(a.positions)[pi]
                                 : static_cast<const int64_t*>(a.positions)[pi];
-    const int64_t frac = (int64_t)((uint64_t)pos * a.turns[pair]);
+    const uint64_t turn = (uint64_t)pos * a.turns[pair];
+    const uint32_t quarters = (uint32_t)((turn + (1ull << 61)) >> 62);  // to the nearest
+    const int64_t rest = (int64_t)(turn - ((uint64_t)quarters << 62));
     float s, c;
-    sincospif((float)frac * 1.0842021724855044e-19f, &s, &c);  // 2^-63
-    angles[tok * 2 * half_pad + pair] = c * a.factor;
-    angles[tok * 2 * half_pad + half_pad + pair] = s * a.factor * a.sign;
+    sincospif((float)rest * 1.0842021724855044e-19f, &s, &c);  // 2^-63
+    if (quarters & 1) {  // a quarter further: (c, s) becomes (-s, c)
+      const float t = c;
+      c = -s;
+      s = t;
+    }
+    const float f = (quarters & 2) ? -a.factor : a.factor;
+    angles[tok * 2 * half_pad + pair] = c * f;
+    angles[tok * 2 * half_pad + half_pad + pair] = s * f * a.sign;
   }
   __syncthreads();
   if (tt >= tg) return;

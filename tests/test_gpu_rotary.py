@@ -10,6 +10,8 @@ f * (|a| + |b|) * (2 pi * 2^-33 + pi * 2^-25 + 2^-23 + 4 * 2^-24), below
 f * (|a| + |b|) * 2^-21, plus eps / 2 of its value for the last rounding.
 """
 
+import math
+
 import pytest
 import torch
 
@@ -148,6 +150,34 @@ def test_overlapping_inputs(interleaved, dtype):
         g = v.clone().requires_grad_()
         gx, = torch.autograd.grad(rotary.apply_rotary(g, None, p, plan)[0], g, v)
         _check(gx, v, p, plan, inv, transpose=True)
+
+
+@pytest.mark.parametrize("start", [0, -3000, 1 << 20, (1 << 40) + 7])
+def test_angles_keep_their_digits(start):
+    """Cosine and sine themselves, of pairs (1, 0) in float32, against whole-number
+    turns.  The rest to the nearest quarter turn is rounded to float32 (2^-24 of it,
+    and as much of its sine at most), sincospif is within 2 ulp (2^-22), the factor 1
+    and the products with 1 and 0 add nothing: 5/4 of 2^-22 of the value, next to 0
+    as well."""
+    plan = rotary.rotary_plan(64, theta=500.0)
+    pos = start + torch.arange(2000, device="cuda")
+    x = torch.zeros((1, 1, 2000, 64), device="cuda")
+    x[..., :32] = 1
+    y = rotary.apply_rotary(x, None, pos, plan)[0][0, 0].double().cpu()
+    near = 1.0
+    for i, w in enumerate(plan.turns.tolist()):
+        turn = [(p * w) % (1 << 64) for p in pos.tolist()]
+        quarters = [((t + (1 << 61)) >> 62) & 3 for t in turn]
+        rest = torch.tensor([(t - (q << 62) + (1 << 63)) % (1 << 64) - (1 << 63)
+                             for t, q in zip(turn, quarters)], dtype=torch.float64)
+        ang = rest * (math.pi * 2.0 ** -63)
+        c, s, q = ang.cos(), ang.sin(), torch.tensor(quarters)
+        cos = torch.where(q == 0, c, torch.where(q == 1, -s, torch.where(q == 2, -c, s)))
+        sin = torch.where(q == 0, s, torch.where(q == 1, c, torch.where(q == 2, -s, -c)))
+        for got, want in ((y[:, i], cos), (y[:, 32 + i], sin)):
+            assert bool(((got - want).abs() <= 1.25 * 2.0 ** -22 * want.abs() + 2.0 ** -149).all())
+            near = min(near, float(want[want != 0].abs().min()))
+    assert near < 1e-3  # some of them do lie next to 0
 
 
 def test_gradient_is_the_transposed_map():
