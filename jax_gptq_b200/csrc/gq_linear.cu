@@ -406,7 +406,7 @@ int run_few(const Args& a, int granule, bool dependent, cudaStream_t st) {
   // keeps a block: 1 token of 1024 x 8192 3.5 us by clusters of 4, 5.5 by single
   // CTAs; of 4096 x 4096 (256 row blocks) 6.8 by pairs, 4.3 without.
   int split = 0;
-  while ((1 << split) < MAX_PARTS && (rbs * groups << split) < 148 && a.nkc >= 2 * WARPS << split) ++split;
+  while ((1 << split) < MAX_PARTS && (rbs * groups << split) < sm_count() && a.nkc >= 2 * WARPS << split) ++split;
   const dim3 grid((unsigned)(rbs << split), (unsigned)groups);
   cudaError_t e;
   if (granule == 128)
@@ -433,7 +433,9 @@ int run_typed(const Args& a, int granule, bool dependent, cudaStream_t st) {
 // The columns of x that the few-token form takes: one CTA's, and 24 where the tcgen05
 // form's row tiles alone fill the SMs.  32 against 33 tokens: 4096 x 4096 9.4 and 12.4
 // us, 11008 x 4096 23.4 and 22.6, 28672 x 8192 94 and 71.
-inline int few_columns(int dtype, int64_t m) { return dtype == 0 || m >= 148 * 128 ? 24 : 32; }
+inline int few_columns(int dtype, int64_t m, int sms) {
+  return dtype == 0 || m >= (int64_t)sms * 128 ? 24 : 32;
+}
 
 inline int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
 
@@ -465,7 +467,7 @@ int gq_linear_layout(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp, 
   const int width = bits <= 4 ? 4 : 8;
   const int64_t rbs = ceil_div(m, lin::ROWS);
   const int64_t words = rbs * lin::ROWS * k * width / 32;
-  const unsigned g1 = (unsigned)std::min<int64_t>(ceil_div(words, 256), 148 * 32);
+  const unsigned g1 = (unsigned)std::min<int64_t>(ceil_div(words, 256), sm_count() * 32);
   if (width == 4)
     lin::layout_codes_kernel<4><<<g1, 256, 0, st>>>(packed, m, ldp, bits, kmap, k / lin::KC, qw, words);
   else
@@ -473,7 +475,7 @@ int gq_linear_layout(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp, 
   GQ_TRY(check_launch("gq_linear_layout codes"));
   const int64_t ngran = k / granule, total = rbs * lin::ROWS * ngran;
   const float qmin = sym ? (float)(1 - (1 << (bits - 1))) : 0.f;
-  lin::layout_params_kernel<<<(unsigned)std::min<int64_t>(ceil_div(total, 256), 148 * 16), 256, 0, st>>>(
+  lin::layout_params_kernel<<<(unsigned)std::min<int64_t>(ceil_div(total, 256), sm_count() * 16), 256, 0, st>>>(
       scales, zeros, m, n_groups, qmin, (float)((1 << bits) - 1), granule_group, ngran,
       reinterpret_cast<float2*>(params), total, bad);
   return check_launch("gq_linear_layout params");
@@ -488,7 +490,7 @@ int gq_test_linear_form(int64_t m, int64_t k, int bits, int granule, int dtype, 
                  sms >= 1,
              "gq_test_linear_form: bad argument");
   for (int i = 0; i < 10; ++i) form[i] = 0;
-  if (tokens * (dtype == 0 ? 3 : 1) > lin::few_columns(dtype, m))
+  if (tokens * (dtype == 0 ? 3 : 1) > lin::few_columns(dtype, m, sms))
     lin::many_form(m, k, bits, granule, dtype, tokens, sms, form);
   return GQ_OK;
 }
@@ -552,7 +554,7 @@ int gq_linear(const uint32_t* qw, const float* params, const int32_t* kmap, int6
     a.x = xp;
     a.ldx = k;
   }
-  if (a.cols > lin::few_columns(dtype, m))
+  if (a.cols > lin::few_columns(dtype, m, sm_count()))
     return lin::run_many(qw, params, m, k, bits, granule, a.x, a.ldx, dtype, tokens, y, ldy, st);
   const bool dep = !in_place;
   if (bits <= 4) {

@@ -195,3 +195,14 @@ def test_weights_of_another_device_are_moved(monkeypatch):
 def test_out_with_a_host_array_is_refused():
     with pytest.raises(ValueError, match="host array"):
         linear.packed_matmul(np.zeros((2, 64), np.float32), None, out=torch.zeros(2, 4))
+
+
+def test_forms_follow_the_number_of_sms():
+    few = (0,) * 10
+    for sms in (100, 132, 148):
+        assert F.form(sms * 128, 512, 4, 128, 1, 25, sms)[0] == 64
+        assert F.form(sms * 128 - 1, 512, 4, 128, 1, 25, sms) == few
+        assert F.form(sms * 128, 512, 4, 128, 1, 24, sms) == few
+    split = lambda m, sms: F.form(m, 8192, 4, 128, 1, 128, sms)[1:4]
+    assert split(14 * 128, 148) == (1, 8, 14) and split(15 * 128, 148) == (1, 4, 15)
+    assert split(12 * 128, 132) == (1, 8, 12) and split(13 * 128, 132) == (1, 4, 13)
