@@ -414,7 +414,7 @@ int gq_unpack_dequant(const uint32_t* packed, int64_t m, int64_t n, int64_t ldp,
  * direct = 1 when kmap is the identity with k == n (16-bit x is then read in
  * place if it is 16-byte aligned with ldx % 8 == 0, and needs no workspace).
  * bits, granule and k as laid out.  Products are summed in float32 in a fixed
- * order and rounded once; float32 x runs as three exact bf16 terms (what lies
+ * order, a granule before its scale (|x| below 2^112), and rounded once; float32 x runs as three exact bf16 terms (what lies
  * below 2^-126 may be lost).  The many-token form has bounded device-side
  * waits: gq_check_device tells whether one expired and left y incomplete.
  * x and y must not overlap.  workspace: 256-byte aligned,

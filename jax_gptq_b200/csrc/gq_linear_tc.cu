@@ -34,10 +34,11 @@
 // leaves its sums in its own shared memory and adds up its share of the columns
 // over the cluster in rank order.  No load uses multicast.
 //
-// Bound: 2048 tokens through 11008 x 4096 take 192 us, 960 TFLOP/s, where cuBLAS on
-// weights already decoded reaches 1426 in a long run and 1686 in a burst: the roles
-// take turns at tensor memory, which three accumulators and two decoded blocks fill.
-// Few tokens (37 float32 ones through 4096 x 4096: 14 us and 3 of the gather) are a
+// Bound: 2048 tokens through 11008 x 4096 take 191 us in a short run with columns in
+// order, 965 TFLOP/s, and 206 to 225 with the gather in long ones, 820 to 900: cuBLAS
+// on weights already decoded takes 133 to 142 (8-bit codes: 225 us in order).  The
+// roles take turns at tensor memory, which three accumulators and two decoded blocks
+// fill.  Few tokens (37 float32 ones through 4096 x 4096: 17 us with the gather) are a
 // chain of about 1600 cycles a block of K.
 //
 // Every wait is bounded (gq_set_wait_limit_ns): one that expires makes all roles
