@@ -749,9 +749,9 @@ inline int most_parts(int nkc) {
 }
 
 // Split K over a cluster while that fills idle SMs and leaves 4 blocks each.  Of
-// clusters of 8, one CTA an SM, 14 run at once on a B200 (they do not cross its groups
-// of SMs), on another part as many of its SMs are taken to be in whole clusters: 128 tokens through 2048 x 8192 (16
-// tiles) take 28.4 us by 8 and 20.7 by 4, through 1792 x 8192 17.0 by 8.
+// clusters of 8, one CTA an SM, 14 run at once on a B200's 148 SMs (they do not cross
+// its groups of SMs), and on other numbers of SMs in proportion: 128 tokens through
+// 2048 x 8192 (16 tiles) take 28.4 us by 8 and 20.7 by 4, through 1792 x 8192 17.0 by 8.
 inline int choose_split(int64_t tiles, int nkc, int sms) {
   const int most = most_parts(nkc);
   int split = 1;

@@ -142,8 +142,7 @@ def packed_matmul(x, w: PreparedLinear, out: torch.Tensor | None = None):
     its scale, so |x| has to stay below 2^112.  numpy in -> numpy out.
     ``out``, if given, is a contiguous tensor of the result's shape and type
     that does not share memory with ``x`` (under ``torch.no_grad()`` where it asks
-    for gradients).  There is no gradient: an ``x`` that
-    asks for one is refused.
+    for gradients).  There is no gradient: an ``x`` that asks for one is refused.
 
     Waits inside the kernel are bounded.  One that expired leaves the result
     incomplete and a status word behind, which this call does not read (it

@@ -353,12 +353,13 @@ class TinyLM(torch.nn.Module):
     @torch.no_grad()
     def generate(self, ids: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
                  min_p=0.0) -> sampling.Sampled:
-        """Continue the prompts ``ids`` [B, T] by one token per column of the
-        uniform numbers ``u`` [B, new], chosen as ``sampling.sample_tokens``
-        does; returns tokens and log-probabilities [B, new].  A row that is
-        left without a token (NaN logits) goes on from token 0.  Waits for the
-        device at the end, and raises ``_lib.DeviceTimeout`` where a kernel's
-        bounded wait expired on the way."""
+        """Continue the prompts ``ids`` [B, T], all of one length (no position is
+        padding), by one token per column of the uniform numbers ``u`` [B, new],
+        chosen as ``sampling.sample_tokens`` does; returns tokens and
+        log-probabilities [B, new].  A row that is left without a token (NaN
+        logits) goes on from token 0.  Waits for the device at the end, and
+        raises ``_lib.DeviceTimeout`` where a kernel's bounded wait expired on
+        the way."""
         if ids.dim() != 2 or ids.shape[1] < 1 or u.dim() != 2 or u.shape[0] != ids.shape[0]:
             raise ValueError(f"ids must be [B, T >= 1] and u [B, new], got {tuple(ids.shape)} and "
                              f"{tuple(u.shape)}")

@@ -52,11 +52,11 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     that share of their mass lies; ``min_p`` keeps of those the ones with
     e >= min_p.  The most likely token always stays.  The result is the
     smallest index at which the running sum of the kept e exceeds u times their
-    total.  ``temperature`` 0 takes the first largest logit; others count as
-    at least 1e-37 and at most 1e36.  NaN and -inf
-    logits are never taken; a row with nothing else gives -1 and -inf.  Terms are
-    whole numbers of 2^-45 of the largest (2^-42 for the largest vocabularies): a
-    token below half of that is never drawn.  The results carry no gradients."""
+    total.  ``temperature`` 0 takes the first largest logit; others count as at
+    least 1e-37 and at most 1e36.  NaN and -inf logits are never taken; a row with
+    nothing else gives -1 and -inf.  Terms are whole numbers of 2^-45 of the
+    largest (2^-42 for the largest vocabularies): a token below half of that is
+    never drawn.  The results carry no gradients."""
     dt = _DTYPES.get(logits.dtype)
     if dt is None:
         raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
